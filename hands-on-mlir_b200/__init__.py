@@ -145,6 +145,14 @@ _SIGNATURES = {
     "homGemmResidualLayernormF16": (None, _MEMREF * 2 + [ctypes.c_bool] + _MEMREF * 2 + [c_float]),
     "homLayernormGemmF16NoAlloc": (None, _MEMREF * 6 + [c_float, c_float]),
     "homGemmDeferredLayernormF16": (None, _MEMREF * 3 + [ctypes.c_bool] + _MEMREF * 4 + [c_int64, c_float]),
+    "homQuantizeMxF4F16": (None, _MEMREF + [c_bool] + _MEMREF * 2),
+    "homQuantizeMxF4F32": (None, _MEMREF + [c_bool] + _MEMREF * 2),
+    "homDequantizeMxF4F16": (None, _MEMREF * 3),
+    "homDequantizeMxF4F32": (None, _MEMREF * 3),
+    "homGemmMxF4F16": (None, _MEMREF * 6 + [c_int64, c_float, c_float]),
+    "homRotaryF16": (None, _MEMREF * 4 + [c_bool, c_bool, c_float]),
+    "homRotaryF32": (None, _MEMREF * 4 + [c_bool, c_bool, c_float]),
+    "homRotaryFrequencies": (None, _MEMREF + [c_double, c_int32] + [c_double] * 4),
     "homKernelLaunchCount": (c_int64, []),
     "homOpTimingEnable": (None, [ctypes.c_int]),
     "homOpTimingCollect": (c_int64, [ctypes.POINTER(OpTiming), c_int64]),
@@ -165,6 +173,13 @@ for _op in ("Add", "Sub", "Mul", "Div"):
 
 #: every symbol include/hom_nvgpu_runner_utils.h declares
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))
+
+
+def mxf4_shapes(rows: int, cols: int) -> tuple[tuple[int, int], tuple[int, int, int]]:
+    """Shapes of the codes and the scales (both uint8) of a [rows, cols] matrix in microscaled 4-bit
+    floating point; see include/hom_nvgpu_runner_utils.h."""
+    blocks = -(-cols // 32)
+    return (rows, 16 * blocks), (-(-rows // 128), -(-blocks // 4), 512)
 
 
 class RunnerUtils:
@@ -279,6 +294,44 @@ class RunnerUtils:
     def nvteBertAttentionF16(self, qkv, cu_seqlens, out, scale, headNum):
         self.lib.nvteBertAttentionF16(*_as_args(qkv), *_as_args(cu_seqlens), *_as_args(out), scale,
                                       headNum)
+        self.check()
+
+    def homQuantizeMxF4F16(self, X, Q, S, transposed=False):
+        self.lib.homQuantizeMxF4F16(*_as_args(X), transposed, *_as_args(Q), *_as_args(S))
+        self.check()
+
+    def homQuantizeMxF4F32(self, X, Q, S, transposed=False):
+        self.lib.homQuantizeMxF4F32(*_as_args(X), transposed, *_as_args(Q), *_as_args(S))
+        self.check()
+
+    def homDequantizeMxF4F16(self, Q, S, Out):
+        self.lib.homDequantizeMxF4F16(*_as_args(Q), *_as_args(S), *_as_args(Out))
+        self.check()
+
+    def homDequantizeMxF4F32(self, Q, S, Out):
+        self.lib.homDequantizeMxF4F32(*_as_args(Q), *_as_args(S), *_as_args(Out))
+        self.check()
+
+    def homGemmMxF4F16(self, A, SA, B, SB, C, D, activation=0, alpha=1.0, beta=0.0):
+        self.lib.homGemmMxF4F16(*_as_args(A), *_as_args(SA), *_as_args(B), *_as_args(SB), *_as_args(C),
+                                *_as_args(D), activation, alpha, beta)
+        self.check()
+
+    def homRotaryF16(self, X, positions, frequencies, Out, interleaved=False, backward=False, magnitude=1.0):
+        self.lib.homRotaryF16(*_as_args(X), *_as_args(positions), *_as_args(frequencies), *_as_args(Out),
+                              interleaved, backward, magnitude)
+        self.check()
+
+    def homRotaryF32(self, X, positions, frequencies, Out, interleaved=False, backward=False, magnitude=1.0):
+        self.lib.homRotaryF32(*_as_args(X), *_as_args(positions), *_as_args(frequencies), *_as_args(Out),
+                              interleaved, backward, magnitude)
+        self.check()
+
+    def homRotaryFrequencies(self, Out, base=10000.0, scaling="none", factor=1.0, original_length=0.0,
+                             beta_fast=32.0, beta_slow=1.0):
+        """`scaling`: "none", "linear", "base" or "parts"."""
+        kind = ("none", "linear", "base", "parts").index(scaling)
+        self.lib.homRotaryFrequencies(*_as_args(Out), base, kind, factor, original_length, beta_fast, beta_slow)
         self.check()
 
     def elementwise(self, op: str, dtype: str, A, B, Out):

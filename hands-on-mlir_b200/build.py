@@ -42,8 +42,12 @@ RUNNER_SOURCES = [
     "attention_sm100.cu",
     "attention_pingpong_sm100.cu",
     "bandwidth_kernels.cu",
+    "mxf4_convert.cu",
+    "gemm_mxf4_sm100.cu",
+    "rotary.cu",
     "runner_utils.cu",
     "no_alloc_entry.cu",
+    "mxf4_rotary_entry.cu",
 ]
 REPLAY_SOURCES = ["bert_replay.cpp", "model_loader.cpp"]
 

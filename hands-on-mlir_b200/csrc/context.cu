@@ -351,6 +351,8 @@ const char *op_kind_name(OpKind kind) {
     case kOpElementwise: return "hom.elementwise";
     case kOpGather: return "hom.gather";
     case kOpCuSeqLen: return "hom.cu_seqlen";
+    case kOpConvert: return "hom.convert";
+    case kOpRotary: return "hom.rotary";
   }
   return "hom.op";
 }

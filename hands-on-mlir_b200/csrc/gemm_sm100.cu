@@ -556,6 +556,41 @@ bool make_tensor_map_2d(const void *ptr, uint64_t inner, uint64_t outer, uint32_
   return true;
 }
 
+bool make_tensor_map_scales(const void *ptr, uint64_t tile_cols, uint64_t tile_rows, uint32_t box_cols,
+                            uint32_t box_rows, CUtensorMap *out) {
+  MapKey key{ptr, tile_cols, tile_rows, box_cols | 0x40000000u, box_rows, 0};
+  {
+    std::lock_guard<std::mutex> lock(g_map_mutex);
+    auto it = g_map_cache.find(key);
+    if (it != g_map_cache.end()) {
+      *out = it->second;
+      return true;
+    }
+  }
+  EncodeFn encode = get_encode_fn();
+  if (!encode) {
+    set_error(HOM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    return false;
+  }
+  cuuint64_t dims[3] = {256, tile_cols, tile_rows};  // in two-byte elements
+  cuuint64_t strides[2] = {512, tile_cols * 512};
+  cuuint32_t box[3] = {256, box_cols, box_rows};
+  cuuint32_t elem_strides[3] = {1, 1, 1};
+  CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(ptr), dims, strides, box,
+                      elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(HOM_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed (%d) for [%llu x %llu] tiles",
+              static_cast<int>(r), static_cast<unsigned long long>(tile_rows),
+              static_cast<unsigned long long>(tile_cols));
+    return false;
+  }
+  std::lock_guard<std::mutex> lock(g_map_mutex);
+  if (g_map_cache.size() > 8192) g_map_cache.clear();
+  g_map_cache.emplace(key, *out);
+  return true;
+}
+
 // Row-major fp16 matrix [rows, cols] with cols % 64 == 0, seen as a 3-D tensor
 // (64 columns, rows, cols / 64 column groups): one box of (64, box_rows, groups) lands in
 // shared memory as `groups` consecutive 128-byte-swizzled [box_rows x 64] sub-tiles, so one

@@ -114,6 +114,11 @@ void profile_report(const char *what, int tiles, int grid, int num_kb, cudaStrea
 bool make_tensor_map_2d(const void *ptr, uint64_t inner, uint64_t outer, uint32_t box_inner,
                         uint32_t box_outer, CUtensorMap *out, uint64_t pitch = 0);
 
+// The scales of a 4-bit operand, [row tiles, column tiles, 512 bytes]: one box is `box_cols` tiles
+// of `box_rows` row tiles, contiguous and unswizzled; tiles beyond the ends arrive as zeros.
+bool make_tensor_map_scales(const void *ptr, uint64_t tile_cols, uint64_t tile_rows, uint32_t box_cols,
+                            uint32_t box_rows, CUtensorMap *out);
+
 // Row-major [rows, cols] fp16 matrix, cols % 64 == 0, as (64, rows, cols/64): one box of
 // (64, box_rows, groups) becomes `groups` consecutive swizzled [box_rows x 64] sub-tiles.
 bool make_tensor_map_grouped(const void *ptr, uint64_t cols, uint64_t rows, uint32_t box_rows,

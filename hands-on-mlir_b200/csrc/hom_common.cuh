@@ -72,6 +72,8 @@ enum OpKind : int32_t {
   kOpElementwise = 4,
   kOpGather = 5,
   kOpCuSeqLen = 6,
+  kOpConvert = 7,
+  kOpRotary = 8,
 };
 
 cudaStream_t current_stream();

@@ -1,0 +1,355 @@
+// Values to microscaled 4-bit floating point and back (format: mxf4_sm100.cuh).
+//
+// For a block of 32 values with largest magnitude a the scale is 2^(floor(log2 a) - 2), the power
+// of two that puts a between 4 and 8, and every value over the scale is rounded to the nearest
+// 4-bit number, ties to even, magnitudes above 6 to 6.  With the fp32 exponent field f of a the
+// scale byte is max(f - 2, 0) and its reciprocal has the exponent field 254 - byte: both exact, so
+// is the product with the value (a result too small for fp32 is far below the 0.25 that rounds to
+// 0), and the only rounding is the one to four bits.
+//
+// Both directions move bytes and nothing else counts: 2.53 (fp16) or 4.53 (fp32) a value.
+#include "bandwidth_kernels.cuh"
+#include "mxf4_sm100.cuh"
+#include "ptx_sm100.cuh"
+
+namespace hom {
+namespace mxf4 {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kLaneValues = 8;                     // consecutive values of a row that a lane holds
+constexpr int kSegment = 32 * kLaneValues;         // a warp's part of a row: 8 blocks, 2 scale tiles wide
+constexpr int kRowStep = kTileRows / 4;            // a warp works on rows r, r + 32, r + 64, r + 96
+
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The scale byte of a block whose largest magnitude has these bits (NaN and infinity compare
+// above every number).
+__device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
+  const uint32_t field = bits >> 23;
+  return field == 255u ? 255u : field < 2u ? 0u : field - 2u;
+}
+
+__device__ __forceinline__ float reciprocal_scale(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0u : (254u - byte) << 23);
+}
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fffffffu : byte << 23);
+}
+
+// Eight values to eight codes, the first in the lowest bits.
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t"
+      "}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+__device__ __forceinline__ void decode8(uint32_t codes, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t"
+      ".reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t"
+      "}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ void load8(const __half *p, float (&v)[8]) {
+  const uint4 raw = *reinterpret_cast<const uint4 *>(p);
+  const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(h[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void store8(__half *p, const float (&v)[8]) {
+  uint4 raw;
+  __half2 *h = reinterpret_cast<__half2 *>(&raw);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<uint4 *>(p) = raw;
+}
+__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
+  reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store1(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store1(float *p, float v) { *p = v; }
+
+// One warp converts a segment of 256 columns of the rows r, r + 32, r + 64 and r + 96 of a
+// 128-row group: four independent loads in flight, and the scales of the four rows are the 16
+// consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED:
+// rows start on 16 bytes (cols % 8 == 0); otherwise the warp reads element by element, coalesced,
+// and sorts the values through shared memory.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kWarps)
+quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales,
+                     long long rows, int cols, int blocks, int segments, long long units) {
+  __shared__ float sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 4 : kSegment];
+  hom::ptx::pdl_launch_dependents();
+  hom::ptx::pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  if (unit >= units) return;
+  const long long group = unit / segments / kRowStep;
+  const int segment = static_cast<int>(unit % segments);
+  const int r = static_cast<int>(unit / segments % kRowStep);
+  const long long row0 = group * kTileRows + r;
+  const int col = segment * kSegment + lane * kLaneValues;
+
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = row0 + i * kRowStep;
+    if (ALIGNED) {
+      if (row < rows && col < cols) {
+        load8(x + row * cols + col, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = segment * kSegment + j * 32 + lane;
+        v[i][j] = row < rows && c < cols ? to_float(x[row * cols + c]) : 0.f;
+      }
+    }
+  }
+  if (!ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sorted[warp][j * 32 + lane] = v[i][j];
+      __syncwarp();
+      load8(&sorted[warp][lane * kLaneValues], v[i]);
+      __syncwarp();
+    }
+  }
+  uint32_t words[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits = max(bits, magnitude_bits(v[i][j]));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+    const uint32_t byte = scale_byte(bits);
+    const float inv = reciprocal_scale(byte);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = byte == 255u ? 0.f : v[i][j] * inv;
+    const long long row = row0 + i * kRowStep;
+    if (row < rows && col < blocks * kBlock)
+      *reinterpret_cast<uint32_t *>(codes + row * (blocks * 16LL) + col / 2) = encode8(v[i]);
+    // the bytes of four neighbouring blocks become the word of one scale tile
+    uint32_t word = byte << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    words[i] = word;
+  }
+  const int tile_cols = (blocks + kTileBlocks - 1) / kTileBlocks;
+  const int tile = segment * 2 + (lane >> 4);
+  if ((lane & 15) == 0 && tile < tile_cols)
+    *reinterpret_cast<uint4 *>(scales + (group * tile_cols + tile) * kTileBytes + r * 16) =
+        make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+// x stored [cols, rows]: a thread owns one row of the result, that is one column of x, for one
+// scale tile (128 values, read 32 at a time: neighbouring threads read neighbouring elements).
+template <typename T>
+__global__ void __launch_bounds__(kTileRows)
+quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales,
+                        long long rows, int cols, int blocks) {
+  hom::ptx::pdl_launch_dependents();
+  hom::ptx::pdl_wait();
+  const int t = threadIdx.x;
+  const long long row = static_cast<long long>(blockIdx.x) * kTileRows + t;
+  const int tile = blockIdx.y, tile_cols = gridDim.y;
+  uint32_t word = 0;
+#pragma unroll
+  for (int b = 0; b < kTileBlocks; ++b) {
+    const int block = tile * kTileBlocks + b;
+    float v[kBlock];
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) {
+      const int c = block * kBlock + j;
+      v[j] = row < rows && c < cols ? to_float(x[c * rows + row]) : 0.f;
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(v[j]));
+    const uint32_t byte = scale_byte(bits);
+    const float inv = reciprocal_scale(byte);
+    uint32_t packed[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float part[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[j] = byte == 255u ? 0.f : v[q * 8 + j] * inv;
+      packed[q] = encode8(part);
+    }
+    if (row < rows && block < blocks)
+      *reinterpret_cast<uint4 *>(codes + (row * blocks + block) * 16) =
+          make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    word |= byte << (8 * b);
+  }
+  *reinterpret_cast<uint32_t *>(scales + (static_cast<long long>(blockIdx.x) * tile_cols + tile) * kTileBytes +
+                                (t & 31) * 16 + (t >> 5) * 4) = word;
+}
+
+// The way back, with the same division of work.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kWarps)
+dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *out,
+                  long long rows, int cols, int blocks, int segments, long long units) {
+  __shared__ float sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 4 : kSegment];
+  hom::ptx::pdl_launch_dependents();
+  hom::ptx::pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  if (unit >= units) return;
+  const long long group = unit / segments / kRowStep;
+  const int segment = static_cast<int>(unit % segments);
+  const int r = static_cast<int>(unit / segments % kRowStep);
+  const long long row0 = group * kTileRows + r;
+  if (row0 >= rows) return;
+  const int col = segment * kSegment + lane * kLaneValues;
+  const int tile_cols = (blocks + kTileBlocks - 1) / kTileBlocks;
+  const int tile = segment * 2 + (lane >> 4);
+
+  uint32_t packed[4], words[4] = {0, 0, 0, 0};
+  if (tile < tile_cols) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(scales + (group * tile_cols + tile) * kTileBytes + r * 16);
+    words[0] = w.x, words[1] = w.y, words[2] = w.z, words[3] = w.w;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = row0 + i * kRowStep;
+    packed[i] = row < rows && col < blocks * kBlock
+                    ? *reinterpret_cast<const uint32_t *>(codes + row * (blocks * 16LL) + col / 2)
+                    : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = row0 + i * kRowStep;
+    if (row >= rows) break;  // the same for the whole warp
+    const float scale = scale_value((words[i] >> (8 * ((lane >> 2) & 3))) & 255u);
+    float v[8];
+    decode8(packed[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
+    T *dst = out + row * cols;
+    if (ALIGNED) {
+      if (col < cols) store8(dst + col, v);
+    } else {
+      __syncwarp();
+      store8(&sorted[warp][lane * kLaneValues], v);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = segment * kSegment + j * 32 + lane;
+        if (c < cols) store1(dst + c, sorted[warp][j * 32 + lane]);
+      }
+    }
+  }
+}
+
+bool grid_fits(long long grid, const char *what) {
+  if (grid <= INT32_MAX) return true;
+  set_error(HOM_ERR_UNSUPPORTED, "%s: the matrix needs more than 2^31 - 1 thread blocks", what);
+  return false;
+}
+
+bool is_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+double traffic(int64_t rows, int64_t cols, size_t element) {
+  return static_cast<double>(rows) * (static_cast<double>(cols) * element + 16.5 * blocks_of(cols));
+}
+
+}  // namespace
+
+template <typename T>
+bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t cols,
+              cudaStream_t stream) {
+  const char *what = "4-bit quantisation launch";
+  const int64_t blocks = blocks_of(cols), tile_rows = tile_rows_of(rows);
+  const long long rows_ll = rows;
+  const int cols_i = static_cast<int>(cols), blocks_i = static_cast<int>(blocks);
+  if (transposed) {
+    const int64_t tile_cols = tile_cols_of(blocks);
+    if (!grid_fits(tile_rows, what)) return false;
+    if (tile_cols > 65535) {
+      set_error(HOM_ERR_UNSUPPORTED, "%s: a transposed matrix has at most 65535 x 128 values along K", what);
+      return false;
+    }
+    LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
+    return check_cuda(launch_pdl(quantize_columns_kernel<T>,
+                                 dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>(tile_cols)),
+                                 dim3(kTileRows), 0, stream, 1, x, codes, scales, rows_ll, cols_i, blocks_i),
+                      what);
+  }
+  const int64_t segments = (cols + kSegment - 1) / kSegment;
+  const long long units = tile_rows * kRowStep * segments;
+  const long long grid = (units + kWarps - 1) / kWarps;
+  if (!grid_fits(grid, what)) return false;
+  auto kernel = cols % kLaneValues == 0 && is_aligned16(x) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+  LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
+  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, x, codes,
+                               scales, rows_ll, cols_i, blocks_i, static_cast<int>(segments), units),
+                    what);
+}
+
+template <typename T>
+bool dequantize(const uint8_t *codes, const uint8_t *scales, T *out, int64_t rows, int64_t cols,
+                cudaStream_t stream) {
+  const char *what = "4-bit dequantisation launch";
+  const int64_t blocks = blocks_of(cols), segments = (cols + kSegment - 1) / kSegment;
+  const long long units = tile_rows_of(rows) * kRowStep * segments;
+  const long long grid = (units + kWarps - 1) / kWarps;
+  if (!grid_fits(grid, what)) return false;
+  auto kernel = cols % kLaneValues == 0 && is_aligned16(out) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+  LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
+  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, codes,
+                               scales, out, static_cast<long long>(rows), static_cast<int>(cols),
+                               static_cast<int>(blocks), static_cast<int>(segments), units),
+                    what);
+}
+
+template bool quantize<__half>(const __half *, bool, uint8_t *, uint8_t *, int64_t, int64_t, cudaStream_t);
+template bool quantize<float>(const float *, bool, uint8_t *, uint8_t *, int64_t, int64_t, cudaStream_t);
+template bool dequantize<__half>(const uint8_t *, const uint8_t *, __half *, int64_t, int64_t, cudaStream_t);
+template bool dequantize<float>(const uint8_t *, const uint8_t *, float *, int64_t, int64_t, cudaStream_t);
+
+}  // namespace mxf4
+}  // namespace hom

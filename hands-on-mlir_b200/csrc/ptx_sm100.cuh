@@ -285,6 +285,31 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, 
       : "memory");
 }
 
+// D[tmem] (+)= (A[smem] * scales) * (B[smem] * scales) for 4-bit operands, M x N x 64 per
+// instruction, one power-of-two scale for every 32 values along K.  Scales lie in tensor memory:
+// row r's four scales of 128 values are the bytes of the 32-bit word at lane r % 32 (repeated in
+// every lane quarter), column r / 32; the instruction descriptor says which two of the four apply.
+__device__ __forceinline__ void tc_mma_mxf4_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                               uint32_t tmem_scales_a, uint32_t tmem_scales_b,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_scales_a), "r"(tmem_scales_b), "r"(accumulate)
+      : "memory");
+}
+
+// 512 contiguous bytes of shared memory, 16 for each of 32 lanes, to four columns of tensor
+// memory, repeated in every lane quarter: one tile of scales.  Executes in order with the MMAs of
+// the issuing thread.
+__device__ __forceinline__ void tc_copy_scales(uint32_t tmem_dst, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+}
+
 // 32 lanes x 32 consecutive fp32 columns: thread t of the warp receives row
 // (lane base of the warp's TMEM quarter + t), columns [col, col + 32).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -468,6 +493,21 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr, uin
   d |= 1ull << 46;
   d |= 2ull << 61;
   return d;
+}
+
+// Instruction descriptor for kind::mxf4 (E2M1 operands, UE8M0 scales, fp32 accumulate, both
+// operands K-major); `pair` 0 or 1: the first or second two scales of the words in tensor memory.
+//   bits [4,6) / [29,31) byte of B's / A's scales   bits [7,10) / [10,12) A / B format (1 = E2M1)
+//   bits [17,23) N >> 3    bit 23 scale format (1 = UE8M0)    bits [24,29) M >> 4
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int pair) {
+  return (static_cast<uint32_t>(2 * pair) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(2 * pair) << 29);
+}
+
+// Shared-memory descriptor of one tile of scales for tc_copy_scales: rows of 16 bytes, eight rows
+// to 128 bytes, no swizzle.
+__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
 }
 
 // The descriptor of the operand `bytes` further on (a multiple of 16; same tile layout).

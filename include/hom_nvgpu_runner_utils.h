@@ -287,13 +287,77 @@ HOM_EXPORT void homLayernormGemmF16NoAlloc(int64_t rankA, void *dstA, int64_t ra
                                            int64_t rankVar, void *dstVar, int64_t rankMean,
                                            void *dstMean, float alpha, float beta);
 
+/* Microscaled 4-bit floating point: 32 consecutive values along K share a power of two, each is one
+ * of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it.  A matrix [rows, K] is held as two uint8 memrefs:
+ *   Q  [.., rows, 16 * ceil(K / 32)]: two codes to a byte, the even column in the low half (sign,
+ *      two exponent bits, one mantissa bit); columns beyond K are 0;
+ *   S  [ceil(rows / 128), ceil(ceil(K / 32) / 4), 512]: the scale byte s of row r and block b,
+ *      meaning 2^(s - 127) (255: NaN), is byte (r % 32) * 16 + (r / 32) % 4 * 4 + b % 4 of tile
+ *      (r / 128, b / 4); bytes of rows and blocks beyond the matrix are 0.
+ * Both 16-byte aligned.  Leading dimensions of a rank-3 operand count as rows.  K and rows may be
+ * anything from 1 to 2^30; a matrix without elements is a call without effect.  An output must not
+ * overlap another operand (C may be D).
+ *
+ * homQuantizeMxF4*: the block's power of two is 2^(floor(log2 max|x|) - 2), at least 2^-127; values
+ * over it are rounded to the nearest code, ties to even, magnitudes above 6 to 6.  A block that
+ * holds a NaN or an infinity becomes NaN as a whole.  X [.., rows, K] (any element alignment), or
+ * [K, rows] / [1, K, rows] with `transposed` (a weight stored [1,K,N]): the blocks run along K
+ * either way.  All of Q and S is written.
+ * homDequantizeMxF4*: Out [.., rows, K] = the values; exact in fp32, in fp16 wherever the values
+ * came from fp16.
+ * No counterpart in the reference, whose path is fp16 throughout. */
+HOM_EXPORT void homQuantizeMxF4F16(int64_t rankX, void *dstX, bool transposed, int64_t rankQ, void *dstQ,
+                                   int64_t rankS, void *dstS);
+HOM_EXPORT void homQuantizeMxF4F32(int64_t rankX, void *dstX, bool transposed, int64_t rankQ, void *dstQ,
+                                   int64_t rankS, void *dstS);
+HOM_EXPORT void homDequantizeMxF4F16(int64_t rankQ, void *dstQ, int64_t rankS, void *dstS, int64_t rankOut,
+                                     void *dstOut);
+HOM_EXPORT void homDequantizeMxF4F32(int64_t rankQ, void *dstQ, int64_t rankS, void *dstS, int64_t rankOut,
+                                     void *dstOut);
+
+/* D = epilogue(alpha * A.B^T + beta * C) of two such matrices, A [.., M, K] and B [N, K] or
+ * [1, N, K] with equal numbers of blocks: the 4-bit counterpart of nvteGemmF16 with its epilogue
+ * (fp32 accumulation; fp16 C and D; C [.., M, N], which may be D, or one row of N; unused when
+ * beta == 0; `activation` 1 = erf GELU).  D (and C) 16-byte aligned when N % 8 == 0.  Q and S of
+ * the weight may be declared (homDeclareWeights, one declaration each) to be fetched early. */
+HOM_EXPORT void homGemmMxF4F16(int64_t rankA, void *dstA, int64_t rankSA, void *dstSA, int64_t rankB,
+                               void *dstB, int64_t rankSB, void *dstSB, int64_t rankC, void *dstC,
+                               int64_t rankD, void *dstD, int64_t activation, float alpha, float beta);
+
+/* Rotary positions.  The first 2F dimensions of every head, F = entries of Frequencies, are F pairs
+ * (i, F + i), or (2i, 2i + 1) with `interleaved`; pair i of a token at position p is turned by
+ * p * Frequencies[i] radians and multiplied by `magnitude`:
+ *   y0 = magnitude * (x0 cos - x1 sin),   y1 = magnitude * (x1 cos + x0 sin).
+ * `backward` applies the transpose, which takes the gradient of Out to that of X.  Dimensions
+ * beyond 2F are copied.  X, Out [bs, seq, heads, d] with any non-negative strides and a contiguous
+ * last dimension - the query and key heads of a packed [bs, seq, 3*heads*d] are the view
+ * [bs, seq, 2*heads, d] of it -; Out may be X, otherwise they must not overlap.  Positions int64
+ * [bs, seq] or [1, seq], absent (rank 0 / null): 0 .. seq - 1.  Frequencies fp64 [F], F <= 512;
+ * angles are formed in 64 bits, so that far positions keep their fractions of a turn.  The
+ * rotation is fp32, rounded once.
+ * No counterpart in the reference, whose model adds a position table. */
+HOM_EXPORT void homRotaryF16(int64_t rankX, void *dstX, int64_t rankPos, void *dstPos, int64_t rankFreq,
+                             void *dstFreq, int64_t rankOut, void *dstOut, bool interleaved, bool backward,
+                             float magnitude);
+HOM_EXPORT void homRotaryF32(int64_t rankX, void *dstX, int64_t rankPos, void *dstPos, int64_t rankFreq,
+                             void *dstFreq, int64_t rankOut, void *dstOut, bool interleaved, bool backward,
+                             float magnitude);
+/* Fills Frequencies (fp64 [F], on the device) with f_i = base^(-i / F).  `scaling` for contexts that
+ * are `factor` times longer: 0 none; 1 linear: f_i / factor; 2 changed base: base * factor^(F / (F - 1))
+ * instead of base, which leaves the fastest pair alone and slows the slowest by factor; 3 by parts:
+ * a pair that makes t = originalLength * f_i / (2 pi) turns keeps the share
+ * g = clamp((t - betaSlow) / (betaFast - betaSlow), 0, 1) of its frequency and has the rest divided:
+ * f_i * (g + (1 - g) / factor). */
+HOM_EXPORT void homRotaryFrequencies(int64_t rankFreq, void *dstFreq, double base, int32_t scaling, double factor,
+                                     double originalLength, double betaFast, double betaSlow);
+
 /* Number of kernels this library has launched since load (all threads). */
 HOM_EXPORT int64_t homKernelLaunchCount(void);
 
 /* Per-launch timing: while enabled every entry point brackets its kernel with events on
  * the current stream.  homOpTimingCollect() synchronises, writes up to `capacity` records
- * (kind: 1 gemm, 2 layernorm, 3 attention, 4 elementwise, 5 gather, 6 cu_seqlen; ms; and
- * the algorithmic flop and byte counts of that launch), clears the log and returns the
+ * (kind: 1 gemm, 2 layernorm, 3 attention, 4 elementwise, 5 gather, 6 cu_seqlen, 7 conversion
+ * to or from 4 bits, 8 rotary; ms; and the algorithmic flop and byte counts of that launch), clears the log and returns the
  * number of records that were available. */
 typedef struct HomOpTiming {
   int32_t kind;
