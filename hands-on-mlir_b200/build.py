@@ -44,6 +44,7 @@ RUNNER_SOURCES = [
     "bandwidth_kernels.cu",
     "mxf4_convert.cu",
     "gemm_mxf4_sm100.cu",
+    "gemm_mxf4_pair_sm100.cu",
     "rotary.cu",
     "runner_utils.cu",
     "no_alloc_entry.cu",

@@ -174,6 +174,7 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }  // namespace
 
 bool run_product(const Problem &pb, cudaStream_t stream) {
+  if (pb.N % 8 == 0 && (pb.M + 255) / 256 * ((pb.N + 255) / 256) >= 16) return run_product_pair(pb, stream);
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -215,10 +216,7 @@ bool run_product(const Problem &pb, cudaStream_t stream) {
     set_error(HOM_ERR_UNSUPPORTED, "4-bit product: more than 2^31 - 1 output tiles");
     return false;
   }
-  const double m = static_cast<double>(pb.M), n = static_cast<double>(pb.N), k = 32.0 * pb.blocks;
-  LaunchScope scope(kOpGemm, 2.0 * m * n * k,
-                    (m + n) * k * (0.5 + 1.0 / kBlock) + 2.0 * m * n * (pb.c_mode == 1 ? 2 : 1) +
-                        (pb.c_mode == 2 ? 2.0 * n : 0.0));
+  LaunchScope scope(kOpGemm, product_flops(pb), product_bytes(pb));
   return check_cuda(launch_pdl(gemm_mxf4_kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kSmemBytes, stream,
                                1, tmA, tmB, tmSA, tmSB, tmD, p),
                     "4-bit product launch");

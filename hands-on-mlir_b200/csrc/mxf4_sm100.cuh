@@ -47,7 +47,15 @@ struct Problem {
   float alpha = 1.f, beta = 0.f;
   int act = 0;  // 1 = erf GELU
 };
+// What the product cannot do without.
+inline double product_flops(const Problem &pb) { return 64.0 * pb.M * pb.N * pb.blocks; }
+inline double product_bytes(const Problem &pb) {
+  return (static_cast<double>(pb.M) + pb.N) * pb.blocks * 17.0 + 2.0 * pb.M * pb.N * (pb.c_mode == 1 ? 2 : 1) +
+         (pb.c_mode == 2 ? 2.0 * pb.N : 0.0);
+}
 bool run_product(const Problem &pb, cudaStream_t stream);
+// On persistent CTA pairs, 256 x 256 tiles (gemm_mxf4_pair_sm100.cu); needs N % 8 == 0.
+bool run_product_pair(const Problem &pb, cudaStream_t stream);
 
 }  // namespace mxf4
 }  // namespace hom

@@ -459,6 +459,27 @@ __device__ __forceinline__ void tc_mma_f16_ss_pair(uint32_t tmem_d, uint64_t des
       : "memory");
 }
 
+// The 4-bit form: A's scales of the 128 rows of each CTA in its own tensor memory, B's scales of all
+// N columns in both, at the same columns.
+__device__ __forceinline__ void tc_mma_mxf4_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                                    uint32_t idesc, uint32_t tmem_scales_a,
+                                                    uint32_t tmem_scales_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_scales_a), "r"(tmem_scales_b), "r"(accumulate)
+      : "memory");
+}
+
+// tc_copy_scales in both CTAs at once, each from its own shared memory to its own tensor memory.
+__device__ __forceinline__ void tc_copy_scales_pair(uint32_t tmem_dst, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+}
+
 // Arrives, in every CTA named by `cta_mask`, on the mbarrier at this shared-memory offset
 // once all MMAs issued so far by this thread have completed.
 __device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t cta_mask) {
