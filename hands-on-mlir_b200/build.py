@@ -45,6 +45,7 @@ RUNNER_SOURCES = [
     "mxf4_convert.cu",
     "gemm_mxf4_sm100.cu",
     "gemm_mxf4_pair_sm100.cu",
+    "gemm_mxf4_rows.cu",
     "rotary.cu",
     "runner_utils.cu",
     "no_alloc_entry.cu",

@@ -66,7 +66,8 @@ static_assert(kScales + 2 * kScaleSet <= kTmemCols, "accumulators and scales exc
 static_assert(kSmemBytes <= 227 * 1024, "exceeds a CTA's shared memory");
 
 struct Params {
-  const __half *C;  // the row of N, when C is one
+  const __half *C;  // read where TMA does not: a row of N; a matrix of kRagged
+  __half *D;        // written by kRagged
   float alpha, beta;
   int c_mode, act;
   int M, N;
@@ -76,8 +77,51 @@ struct Params {
   int *status;
 };
 
-// Which C and activation an instantiation handles, with alpha = beta = 1; kAny handles all of it.
-enum Form { kNone = 0, kRow = 1, kFull = 2, kGelu = 4, kAny = 8 };
+// Which C and activation an instantiation handles, with alpha = beta = 1; kAny handles all of it,
+// kRagged also N that is not a multiple of 8: rows of C and D then start at any element, and the
+// warp moves them between memory and its staging tile itself, a row at a time.
+enum Form { kNone = 0, kRow = 1, kFull = 2, kGelu = 4, kAny = 8, kRagged = 16 };
+__host__ __device__ constexpr bool general(int form) { return form == kAny || form == kRagged; }
+
+// The staging tile of 32 rows x 64 columns: 128-byte rows whose 16-byte chunks are XOR-swizzled by
+// the row; this lane's two neighbouring columns are the 32-bit word at this place.
+__device__ __forceinline__ uint32_t staging_word(uint32_t stage_smem, int row, int lane) {
+  return stage_smem + row * 128 + ((static_cast<uint32_t>(lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4;
+}
+
+// kRagged: C's block to the staging tile, zeros beyond the matrix; eight rows in flight.
+__device__ __forceinline__ void ragged_load(const __half *c, int m, int n, int row0, int c0, uint32_t stage_smem, int lane) {
+  const unsigned short *from = reinterpret_cast<const unsigned short *>(c);
+  const int col = c0 + 2 * lane;
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    uint32_t v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int row = row0 + r0 + r;
+      const unsigned short *at = from + static_cast<long long>(row) * n + col;
+      const uint32_t lo = row < m && col < n ? at[0] : 0u, hi = row < m && col + 1 < n ? at[1] : 0u;
+      v[r] = lo | hi << 16;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(staging_word(stage_smem, r0 + r, lane)), "r"(v[r]) : "memory");
+  }
+}
+
+__device__ __forceinline__ void ragged_store(__half *d, int m, int n, int row0, int c0, uint32_t stage_smem, int lane) {
+  unsigned short *to = reinterpret_cast<unsigned short *>(d);
+  const int col = c0 + 2 * lane;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    const int row = row0 + r;
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(staging_word(stage_smem, r, lane)) : "memory");
+    unsigned short *at = to + static_cast<long long>(row) * n + col;
+    if (row < m && col < n) at[0] = static_cast<unsigned short>(v);
+    if (row < m && col + 1 < n) at[1] = static_cast<unsigned short>(v >> 16);
+  }
+}
 
 // Applies the epilogue to 32 accumulators of this lane's row and leaves the fp16 results in the
 // staging tile, whose row holds C's values where C is a matrix; `bias` is the row of C otherwise.
@@ -85,8 +129,8 @@ template <int FORM>
 __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&acc)[32], int half, uint32_t my_row,
                                             uint32_t bias, int lane) {
   const float2 alpha2 = make_float2(p.alpha, p.alpha), beta2 = make_float2(p.beta, p.beta);
-  const bool full = FORM == kAny ? p.c_mode == 1 : (FORM & kFull) != 0;
-  const bool row = FORM == kAny ? p.c_mode == 2 : (FORM & kRow) != 0;
+  const bool full = general(FORM) ? p.c_mode == 1 : (FORM & kFull) != 0;
+  const bool row = general(FORM) ? p.c_mode == 2 : (FORM & kRow) != 0;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const uint32_t addr = my_row + ((static_cast<uint32_t>(half * 4 + g) ^ (lane & 7u)) << 4);
@@ -103,12 +147,12 @@ __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&ac
     for (int j = 0; j < 4; ++j) {
       const int i = g * 8 + 2 * j;
       float2 v = make_float2(__uint_as_float(acc[i]), __uint_as_float(acc[i + 1]));
-      if (FORM == kAny) v = __fmul2_rn(alpha2, v);
+      if (general(FORM)) v = __fmul2_rn(alpha2, v);
       if (full || row) {
         const float2 cf = __half22float2(*reinterpret_cast<const __half2 *>(&c[j]));
-        v = FORM == kAny ? __ffma2_rn(beta2, cf, v) : __fadd2_rn(cf, v);
+        v = general(FORM) ? __ffma2_rn(beta2, cf, v) : __fadd2_rn(cf, v);
       }
-      if (FORM == kAny ? p.act == 1 : (FORM & kGelu) != 0) v = gelu2(v);
+      if (general(FORM) ? p.act == 1 : (FORM & kGelu) != 0) v = gelu2(v);
       const __half2 h = __floats2half2_rn(v.x, v.y);
       w[j] = *reinterpret_cast<const uint32_t *>(&h);
     }
@@ -312,8 +356,9 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const uint32_t stage_smem = smem_base + kStaging + drain * gemm::kEpilogueStageBytes;
     const uint32_t my_row = stage_smem + lane * 128;
     const uint32_t bias = smem_base + kBias + drain * 128;
-    const bool full = FORM == kAny ? p.c_mode == 1 : (FORM & kFull) != 0;
-    const bool row = FORM == kAny ? p.c_mode == 2 : (FORM & kRow) != 0;
+    const bool full = general(FORM) ? p.c_mode == 1 : (FORM & kFull) != 0;
+    const bool row = general(FORM) ? p.c_mode == 2 : (FORM & kRow) != 0;
+    constexpr bool ragged = FORM == kRagged;
     auto arrive_even = [&](uint32_t bar) {
       if (lane == 0) {
         if (rank == 0) mbar_arrive(bar);
@@ -323,6 +368,11 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     // two neighbouring values of the row of C, requested one tile ahead
     auto load_row = [&](int tile) {
       const int col = tile % p.n_blocks * BN + group * 64 + 2 * lane;
+      if (ragged) {
+        const unsigned short *at = reinterpret_cast<const unsigned short *>(p.C) + col;
+        const uint32_t lo = col < p.N ? at[0] : 0u, hi = col + 1 < p.N ? at[1] : 0u;
+        return lo | hi << 16;
+      }
       return col < p.N ? *reinterpret_cast<const uint32_t *>(p.C + col) : 0u;
     };
     pdl_wait();  // C may be produced, and D still read, by the previous kernel
@@ -334,7 +384,11 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const int c0 = tile % p.n_blocks * BN + group * 64;
       // The staging tile was handed to TMA by this warp's previous block: that read must be over
       // before the tile is written again.
-      if (full && lane == 0) {
+      if (ragged) {
+        __syncwarp();
+        if (full) ragged_load(p.C, p.M, p.N, row0, c0, stage_smem, lane);
+        __syncwarp();
+      } else if (full && lane == 0) {
         bulk_wait_group_read_0();
         mbar_arrive_expect_tx(c_bar(drain), gemm::kEpilogueTileBytes);
         tma_load_2d(stage_smem, &tmC, c_bar(drain), c0, row0);
@@ -355,6 +409,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         __syncwarp();
       };
       auto staging_ready = [&]() {
+        if (ragged) return;
         if (!full) {
           if (lane == 0) bulk_wait_group_read_0();
           __syncwarp();
@@ -388,6 +443,11 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         finish_half<FORM>(p, v, 1, my_row, bias, lane);
       }
       if (!ok) break;
+      if (ragged) {
+        __syncwarp();
+        ragged_store(p.D, p.M, p.N, row0, c0, stage_smem, lane);
+        continue;
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -416,9 +476,10 @@ bool run_product_pair(const Problem &pb, cudaStream_t stream) {
   static const Kernel kernels[] = {gemm_mxf4_pair_kernel<kNone>,        gemm_mxf4_pair_kernel<kRow>,
                                    gemm_mxf4_pair_kernel<kFull>,        gemm_mxf4_pair_kernel<kGelu>,
                                    gemm_mxf4_pair_kernel<kRow | kGelu>, gemm_mxf4_pair_kernel<kFull | kGelu>,
-                                   gemm_mxf4_pair_kernel<kAny>};
+                                   gemm_mxf4_pair_kernel<kAny>,          gemm_mxf4_pair_kernel<kRagged>};
   const bool units = pb.alpha == 1.f && (pb.c_mode == 0 || pb.beta == 1.f);
-  const Kernel kernel = kernels[!units ? 6 : (pb.act ? 3 : 0) + (pb.c_mode == 0 ? 0 : pb.c_mode == 2 ? 1 : 2)];
+  const bool ragged = pb.N % 8 != 0;
+  const Kernel kernel = kernels[ragged ? 7 : !units ? 6 : (pb.act ? 3 : 0) + (pb.c_mode == 0 ? 0 : pb.c_mode == 2 ? 1 : 2)];
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -456,13 +517,15 @@ bool run_product_pair(const Problem &pb, cudaStream_t stream) {
   if (!gemm::make_tensor_map_2d(pb.A, pitch, pb.M, kStepBytes / 2, kHalf, &tmA) ||
       !gemm::make_tensor_map_2d(pb.B, pitch, pb.N, kStepBytes / 2, kHalf, &tmB) ||
       !gemm::make_tensor_map_scales(pb.scales_a, tile_cols, tile_rows_of(pb.M), kStepTiles, 1, &tmSA) ||
-      !gemm::make_tensor_map_scales(pb.scales_b, tile_cols, tile_rows_of(pb.N), kStepTiles, 2, &tmSB) ||
-      !gemm::make_tensor_map_2d(pb.D, pb.N, pb.M, 64, 32, &tmD))
+      !gemm::make_tensor_map_scales(pb.scales_b, tile_cols, tile_rows_of(pb.N), kStepTiles, 2, &tmSB))
     return false;
+  tmD = tmA;  // not used when the rows are ragged
+  if (!ragged && !gemm::make_tensor_map_2d(pb.D, pb.N, pb.M, 64, 32, &tmD)) return false;
   tmC = tmD;
-  if (pb.c_mode == 1 && pb.C != pb.D && !gemm::make_tensor_map_2d(pb.C, pb.N, pb.M, 64, 32, &tmC)) return false;
+  if (!ragged && pb.c_mode == 1 && pb.C != pb.D && !gemm::make_tensor_map_2d(pb.C, pb.N, pb.M, 64, 32, &tmC)) return false;
   Params p = {};
   p.C = pb.C;
+  p.D = pb.D;
   p.alpha = pb.alpha;
   p.beta = pb.beta;
   p.c_mode = pb.c_mode;

@@ -1,15 +1,26 @@
 // Product of two microscaled 4-bit matrices (format: mxf4_sm100.cuh) on the block-scaled tensor
-// path: D = act(alpha * A.B^T + beta * C), fp32 accumulation, fp16 C and D.
+// path, for problems with few output tiles: D = act(alpha * A.B^T + beta * C), fp32 accumulation,
+// fp16 C and D.  And the choice between this form and the others.
 //
-// One CTA per 128 x 128 tile of D.  A K step is 256 values: 128 bytes of codes a row, fetched by
-// TMA into 128-byte-swizzled tiles like the fp16 kernels' 64 values, and two scale tiles for each
-// operand, which tcgen05.cp takes from shared to tensor memory right before the four MMAs that use
-// them.  Zeros that TMA fills in beyond the matrix (codes 0, scales 2^-127) add nothing.
+// A 128 x 64 tile of D belongs to a cluster of one, two or four CTAs that share its K range.  A K step is 256 values: 128 bytes of codes a row, fetched by TMA into 128-byte-swizzled
+// tiles like the fp16 kernels' 64 values, and two scale tiles for each operand, which tcgen05.cp
+// takes from shared to tensor memory right before the four MMAs that use them.  Zeros that TMA fills
+// in beyond the matrix (codes 0, scales 2^-127) add nothing.  A stage of the ring has scales of its
+// own in tensor memory: that the stage was filled again says that the MMAs of its last use, and
+// their reads of the scales, are over.
+//
+// The partial tiles are exchanged SM to SM as in the fp16 cluster kernel (gemm_cluster_sm100.cu):
+// CTA r owns rows [r, r + 1) * ceil(rows / parts) of the tile, every CTA stores its part of them
+// into the owner's shared memory, and after a cluster barrier the owner adds the parts in part order
+// (bit-identical from run to run), applies the epilogue and writes full rows.  What bounds it is
+// latency: launch, first loads, exchange and store one after the other.
 //
 //   warp 0  TMA producer      warp 1  tensor memory, scale copies, MMA issue
-//   warps 2-9  epilogue (gemm_epilogue.cuh), one 32 x 64 block each
-#include "gemm_epilogue.cuh"
+//   warps 2-9  accumulator exchange and epilogue
+#include <atomic>
+
 #include "gemm_sm100.cuh"
+#include "mxf4_epilogue.cuh"
 #include "mxf4_sm100.cuh"
 #include "ptx_sm100.cuh"
 
@@ -17,60 +28,80 @@ namespace hom {
 namespace mxf4 {
 
 using namespace hom::ptx;
-using gemm::EpilogueParams;
 
 namespace {
 
-constexpr int BM = 128, BN = 128;
-constexpr int kStepBytes = 128;                       // of a row of codes: 256 values
-constexpr int kStepBlocks = 2 * kStepBytes / kBlock;  // 8
-constexpr int kStepTiles = kStepBlocks / kTileBlocks; // 2 scale tiles
-constexpr int kMmasPerStep = 4;
+constexpr int BM = 128, BN = 64;
+constexpr int kStepBytes = 128;                        // of a row of codes: 256 values
+constexpr int kStepBlocks = 2 * kStepBytes / kBlock;   // 8
+constexpr int kStepTiles = kStepBlocks / kTileBlocks;  // 2 scale tiles
 constexpr int kStages = 4;
-constexpr int kDrainWarps = 8;
-constexpr int kThreads = 32 * (2 + kDrainWarps);
+constexpr int kExchangeThreads = 256;
+constexpr int kThreads = 64 + kExchangeThreads;
+constexpr int kMaxParts = 4;
 constexpr uint32_t kABytes = BM * kStepBytes, kBBytes = BN * kStepBytes;
 constexpr uint32_t kScaleBytes = kStepTiles * kTileBytes;
 constexpr uint32_t kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
+constexpr uint32_t kRecv = kStages * kStageBytes;
+constexpr uint32_t kBars = kRecv + BM * BN * 4;  // parts * ceil(rows / parts) <= 128 for 1, 2 and 4 parts
+constexpr uint32_t kScaleCols = 4 * kStepTiles;  // tensor-memory columns of one operand's scales
+constexpr uint32_t kTmemCols = 128;
+// All that a CTA can have: no CTA of another kernel may sit beside one of this (gemm_cluster_sm100.cu).
+constexpr uint32_t kSmemBytes = 227 * 1024;
 static_assert(kStageBytes % 1024 == 0, "swizzled tiles start on 1024 bytes");
-constexpr uint32_t kStagingBytes = kDrainWarps * gemm::kEpilogueStageBytes;
-constexpr uint32_t kBarrierBytes = 8 * (2 * kStages + 1) + 16;
-constexpr uint32_t kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarrierBytes + 1024;
-// tensor memory: the accumulator, then the scales of two steps in turn
-constexpr uint32_t kTmemCols = 256;
-constexpr uint32_t kTmemScales = BN, kTmemScalesB = kStepTiles * 4, kTmemScaleSet = 2 * kStepTiles * 4;
+static_assert(kBars + 8 * (2 * kStages + 1) + 16 + 1024 <= kSmemBytes, "exceeds a CTA's shared memory");
+static_assert(BN + kStages * 2 * kScaleCols <= kTmemCols, "accumulator and scales exceed the allocation");
 
 struct Params {
-  EpilogueParams ep;
-  int steps, n_blocks;
+  const __half *C;
+  __half *D;
+  float alpha, beta;
+  int c_mode, act;
+  int M, N, steps, n_blocks;
+  int b_early;  // B is a declared constant: request its tiles before griddepcontrol.wait
   int *status;
 };
 
+__device__ __forceinline__ uint32_t cluster_nctas() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ float2 epilogue2(const Params &p, float2 v, float2 c) {
+  v = __fmul2_rn(make_float2(p.alpha, p.alpha), v);
+  if (p.c_mode != 0) v = __ffma2_rn(make_float2(p.beta, p.beta), c, v);
+  return p.act == 1 ? gelu2(v) : v;
+}
+
+// ALIGNED: N % 8 == 0, rows of C and D travel in 16-byte pieces; otherwise element by element,
+// neighbouring threads at neighbouring columns.
+template <bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                 const __grid_constant__ CUtensorMap tmD, const Params p) {
+                 const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t smem_base = (raw_addr + 1023u) & ~1023u;
   uint8_t *smem_gen = smem_raw + (smem_base - raw_addr);
-  const uint32_t staging_base = smem_base + kStages * kStageBytes;
-  const uint32_t bar_base = staging_base + kStagingBytes;
-  auto full_bar = [&](int s) { return bar_base + 8u * s; };
-  auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
-  const uint32_t acc_bar = bar_base + 8u * (2 * kStages);
-  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kStages * kStageBytes + kStagingBytes +
-                                                                       8 * (2 * kStages + 1));
+  auto full_bar = [&](int s) { return smem_base + kBars + 8u * s; };
+  auto empty_bar = [&](int s) { return smem_base + kBars + 8u * (kStages + s); };
+  const uint32_t acc_bar = smem_base + kBars + 8u * (2 * kStages);
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + kBars + 8 * (2 * kStages + 1));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = static_cast<int>(blockIdx.x) / p.n_blocks * BM, n0 = static_cast<int>(blockIdx.x) % p.n_blocks * BN;
+  const int parts = static_cast<int>(cluster_nctas()), part = static_cast<int>(cluster_ctarank());
+  const int tile = static_cast<int>(blockIdx.x) / parts;
+  const int m0 = tile / p.n_blocks * BM, n0 = tile % p.n_blocks * BN;
+  const int first = part * p.steps / parts;
+  const int steps = (part + 1) * p.steps / parts - first;  // >= 1: the launcher keeps parts <= steps
 
   if (threadIdx.x == 64) {
-    prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
-    prefetch_tensormap(&tmSA);
     prefetch_tensormap(&tmSB);
+    prefetch_tensormap(&tmA);
+    prefetch_tensormap(&tmSA);
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -90,24 +121,37 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();
+  // Cluster barrier, phase 1: "this CTA runs"; its shared memory may be written by its peers.
+  // Every thread of every CTA arrives and waits exactly once per phase, on error paths too.
+  cluster_arrive();
 
   if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
+      auto load_b = [&](uint32_t dst, uint32_t bar, int i) {
+        tma_load_2d(dst + kABytes, &tmB, bar, (first + i) * (kStepBytes / 2), n0);
+        tma_load_3d(dst + kABytes + kBBytes + kScaleBytes, &tmSB, bar, 0, (first + i) * kStepTiles, n0 / kTileRows);
+      };
+      const int early = min(steps, kStages);
+      for (int i = 0; i < early; ++i) {
+        mbar_arrive_expect_tx(full_bar(i), kStageBytes);
+        if (p.b_early) load_b(smem_base + i * kStageBytes, full_bar(i), i);
+      }
       pdl_wait();
       bool ok = true;
-      int armed = 0;
-      for (int i = 0; i < p.steps; ++i) {
+      int armed = early;
+      for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        const uint32_t ph = (i / kStages) & 1;
-        ok = mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, kDevWaitTimeoutProducer);
-        if (!ok) break;
         const uint32_t dst = smem_base + s * kStageBytes;
-        mbar_arrive_expect_tx(full_bar(s), kStageBytes);
-        tma_load_2d(dst, &tmA, full_bar(s), i * (kStepBytes / 2), m0);
-        tma_load_2d(dst + kABytes, &tmB, full_bar(s), i * (kStepBytes / 2), n0);
-        tma_load_3d(dst + kABytes + kBBytes, &tmSA, full_bar(s), 0, i * kStepTiles, m0 / kTileRows);
-        tma_load_3d(dst + kABytes + kBBytes + kScaleBytes, &tmSB, full_bar(s), 0, i * kStepTiles, n0 / kTileRows);
-        ++armed;
+        if (i >= early) {
+          ok = mbar_wait(empty_bar(s), ((i / kStages) & 1) ^ 1, abort_flag, p.status, kDevWaitTimeoutProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(full_bar(s), kStageBytes);
+          ++armed;
+        }
+        if (i >= early || !p.b_early) load_b(dst, full_bar(s), i);
+        tma_load_2d(dst, &tmA, full_bar(s), (first + i) * (kStepBytes / 2), m0);
+        tma_load_3d(dst + kABytes + kBBytes, &tmSA, full_bar(s), 0, (first + i) * kStepTiles, m0 / kTileRows);
       }
       if (!ok) {
         // Let every copy this thread started land before the CTA gives its shared memory back.
@@ -121,45 +165,166 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
     __syncwarp();
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
   } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA issuer
     if (elect_one()) {
+      // the tile may start in the middle of a scale tile
+      const uint32_t shift = n0 % kTileRows / 32;
       bool ok = true;
-      for (int i = 0; i < p.steps; ++i) {
+      for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
         ok = mbar_wait(full_bar(s), (i / kStages) & 1, abort_flag, p.status, kDevWaitTimeoutMma);
         if (!ok) break;
         tc_fence_after_sync();
         const uint32_t src = smem_base + s * kStageBytes;
-        const uint32_t scales = tmem_base + kTmemScales + (i & 1) * kTmemScaleSet;
+        const uint32_t scales = tmem_base + BN + s * 2 * kScaleCols;
 #pragma unroll
         for (int t = 0; t < 2 * kStepTiles; ++t)
           tc_copy_scales(scales + t * 4, make_smem_desc_scales(src + kABytes + kBBytes + t * kTileBytes));
         const uint64_t da = make_smem_desc_sw128(src, 16, 1024), db = make_smem_desc_sw128(src + kABytes, 16, 1024);
 #pragma unroll
-        for (int k = 0; k < kMmasPerStep; ++k)
+        for (int k = 0; k < 2 * kStepTiles; ++k)
           tc_mma_mxf4_ss(tmem_base, smem_desc_advance(da, k * 32), smem_desc_advance(db, k * 32),
                          k & 1 ? make_idesc_mxf4(BM, BN, 1) : make_idesc_mxf4(BM, BN, 0), scales + (k >> 1) * 4,
-                         scales + kTmemScalesB + (k >> 1) * 4, i != 0 || k != 0 ? 1u : 0u);
+                         scales + kScaleCols + (k >> 1) * 4 + shift, i != 0 || k != 0 ? 1u : 0u);
         tc_commit(empty_bar(s));
       }
       if (ok) tc_commit(acc_bar);
     }
     __syncwarp();
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
   } else {
-    const int quarter = warp & 3;
-    const int col_begin = ((warp - 2) >> 2) * 64;
-    uint4 cval[8];
+    // ------------------------------------------- accumulator exchange and epilogue
+    const int rows = min(BM, p.M - m0);               // rows of the tile inside the matrix
+    const int rows_per = (rows + parts - 1) / parts;  // rows each CTA of the cluster finishes
+    const int row_first = part * rows_per;
+    const int my_rows = max(0, min(rows_per, rows - row_first));
+    const int t = threadIdx.x - 64;
+    constexpr int kPieces = BN / 8;  // 8-column pieces of an output row
+    constexpr int kTasks = ALIGNED ? BM * kPieces / kExchangeThreads : 1;
+
     pdl_wait();  // C may be produced, and D still read, by the previous kernel
-    gemm::epilogue_load_c(p.ep, m0 + quarter * 32 + lane, n0 + col_begin, cval);
+    uint4 cval[kTasks];
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < kTasks; ++i) {
+        cval[i] = make_uint4(0, 0, 0, 0);
+        const int row = (t + i * kExchangeThreads) / kPieces, col = n0 + (t + i * kExchangeThreads) % kPieces * 8;
+        if (p.c_mode != 0 && row < my_rows && col < p.N)
+          cval[i] = *reinterpret_cast<const uint4 *>(
+              p.C + (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + row) * p.N : 0) + col);
+      }
+    }
     bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, kDevWaitTimeoutEpilogue);
     ok = __all_sync(0xffffffffu, ok);
+    cluster_wait();  // phase 1: every CTA of the cluster runs
     if (ok) {
       tc_fence_after_sync();
-      gemm::epilogue_warp_block(p.ep, &tmD, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_begin,
-                                m0 + quarter * 32, n0 + col_begin, true, staging_base + (warp - 2) * gemm::kEpilogueStageBytes,
-                                lane, cval, [] {});
-      if (lane == 0) bulk_wait_group_read_0();
-      __syncwarp();
+      const int quarter = warp & 3;
+      const int row = quarter * 32 + lane;
+      const int col_begin = ((warp - 2) >> 2) * (BN / 2);
+      if (quarter * 32 < rows) {  // warp-uniform: the accumulator read is warp-collective
+        const int owner = min(row / rows_per, parts - 1), local = row - owner * rows_per;
+        const uint32_t dst =
+            map_to_cta(smem_base + kRecv + static_cast<uint32_t>(part * rows_per + (row < rows ? local : 0)) * (BN * 4),
+                       static_cast<uint32_t>(owner));
+#pragma unroll
+        for (int h = 0; h < BN / 64; ++h) {
+          uint32_t acc[32];
+          tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_begin + h * 32, acc);
+          tmem_ld_wait();
+          if (row < rows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              // 16-byte chunks of a row are XOR-swizzled by the row: conflict-free stores
+              const uint32_t chunk = static_cast<uint32_t>((col_begin + h * 32) / 4 + j) ^ (local & 7);
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + chunk * 16), "r"(acc[4 * j]),
+                           "r"(acc[4 * j + 1]), "r"(acc[4 * j + 2]), "r"(acc[4 * j + 3])
+                           : "memory");
+            }
+          }
+        }
+        tc_fence_before_sync();
+      }
+    }
+    cluster_arrive();  // phase 2: the parts are delivered
+    cluster_wait();
+    if (ok) {
+      // the sum of the parts, in part order, at (local row, chunk of four columns)
+      auto total = [&](int local, int chunk) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < parts; ++q) {
+          float4 f;
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                       : "r"(smem_base + kRecv + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
+                             (static_cast<uint32_t>(chunk) ^ (local & 7)) * 16)
+                       : "memory");
+          v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+        }
+        return v;
+      };
+      if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < kTasks; ++i) {
+          const int local = (t + i * kExchangeThreads) / kPieces, piece = (t + i * kExchangeThreads) % kPieces;
+          const int col = n0 + piece * 8;
+          if (local < my_rows && col < p.N) {
+            const __half2 *c2 = reinterpret_cast<const __half2 *>(&cval[i]);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float4 v = total(local, 2 * piece + j);
+              const float2 x = epilogue2(p, make_float2(v.x, v.y), __half22float2(c2[2 * j]));
+              const float2 y = epilogue2(p, make_float2(v.z, v.w), __half22float2(c2[2 * j + 1]));
+              const __half2 hx = __floats2half2_rn(x.x, x.y), hy = __floats2half2_rn(y.x, y.y);
+              w[2 * j] = *reinterpret_cast<const uint32_t *>(&hx);
+              w[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&hy);
+            }
+            *reinterpret_cast<uint4 *>(p.D + static_cast<long long>(m0 + row_first + local) * p.N + col) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      } else {
+        // one column per thread, eight rows of C in flight
+        const int column = t % BN, col = n0 + column;
+        const uint32_t at = smem_base + kRecv + (column & 3) * 4;
+        constexpr int kRowStep = kExchangeThreads / BN;
+        if (col < p.N) {
+          for (int base = t / BN; base < my_rows; base += 8 * kRowStep) {
+            float c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int local = base + i * kRowStep;
+              c[i] = p.c_mode != 0 && local < my_rows
+                         ? __half2float(p.C[(p.c_mode == 1 ? static_cast<long long>(m0 + row_first + local) * p.N : 0) + col])
+                         : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int local = base + i * kRowStep;
+              if (local >= my_rows) break;
+              float v = 0.f;
+              for (int q = 0; q < parts; ++q) {
+                float f;
+                asm volatile("ld.shared.f32 %0, [%1];"
+                             : "=f"(f)
+                             : "r"(at + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
+                                   (static_cast<uint32_t>(column >> 2) ^ (local & 7)) * 16)
+                             : "memory");
+                v += f;
+              }
+              p.D[static_cast<long long>(m0 + row_first + local) * p.N + col] =
+                  __float2half_rn(epilogue2(p, make_float2(v, 0.f), make_float2(c[i], 0.f)).x);
+            }
+          }
+        }
+      }
     }
   }
 
@@ -171,55 +336,63 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
 }
 
-}  // namespace
-
-bool run_product(const Problem &pb, cudaStream_t stream) {
-  if (pb.N % 8 == 0 && (pb.M + 255) / 256 * ((pb.N + 255) / 256) >= 16) return run_product_pair(pb, stream);
-  static bool attr_set[64] = {};
+template <bool ALIGNED>
+bool launch(const Problem &pb, int parts, cudaStream_t stream) {
+  static std::atomic<bool> ready[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
-  if (!attr_set[dev]) {
-    if (!check_cuda(cudaFuncSetAttribute(gemm_mxf4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes),
+  auto kernel = gemm_mxf4_kernel<ALIGNED>;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (!check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes),
                     "cudaFuncSetAttribute(4-bit product)"))
       return false;
-    attr_set[dev] = true;
+    ready[dev].store(true, std::memory_order_release);
   }
   const int64_t pitch = pb.blocks * 8;  // in two-byte elements, what the tensor maps count in
   const int64_t tile_cols = tile_cols_of(pb.blocks);
-  const bool unaligned_n = pb.N % 8 != 0;
-  CUtensorMap tmA, tmB, tmSA, tmSB, tmD;
+  CUtensorMap tmA, tmB, tmSA, tmSB;
   if (!gemm::make_tensor_map_2d(pb.A, pitch, pb.M, kStepBytes / 2, BM, &tmA) ||
       !gemm::make_tensor_map_2d(pb.B, pitch, pb.N, kStepBytes / 2, BN, &tmB) ||
-      !gemm::make_tensor_map_scales(pb.scales_a, tile_cols, tile_rows_of(pb.M), kStepTiles, BM / kTileRows, &tmSA) ||
-      !gemm::make_tensor_map_scales(pb.scales_b, tile_cols, tile_rows_of(pb.N), kStepTiles, BN / kTileRows, &tmSB))
+      !gemm::make_tensor_map_scales(pb.scales_a, tile_cols, tile_rows_of(pb.M), kStepTiles, 1, &tmSA) ||
+      !gemm::make_tensor_map_scales(pb.scales_b, tile_cols, tile_rows_of(pb.N), kStepTiles, 1, &tmSB))
     return false;
-  if (unaligned_n) tmD = tmA;  // never dereferenced: the epilogue stores without TMA
-  else if (!gemm::make_tensor_map_2d(pb.D, pb.N, pb.M, 64, 32, &tmD)) return false;
   Params p = {};
-  p.ep.C = pb.C;
-  p.ep.ldc = pb.N;
-  p.ep.c_mode = pb.c_mode;
-  p.ep.D = pb.D;
-  p.ep.ldd = pb.N;
-  p.ep.alpha = pb.alpha;
-  p.ep.beta = pb.beta;
-  p.ep.act = pb.act;
-  p.ep.M = static_cast<int>(pb.M);
-  p.ep.N = static_cast<int>(pb.N);
-  p.ep.unaligned_n = unaligned_n ? 1 : 0;
+  p.C = pb.C;
+  p.D = pb.D;
+  p.alpha = pb.alpha;
+  p.beta = pb.beta;
+  p.c_mode = pb.c_mode;
+  p.act = pb.act;
+  p.M = static_cast<int>(pb.M);
+  p.N = static_cast<int>(pb.N);
   p.steps = static_cast<int>((pb.blocks + kStepBlocks - 1) / kStepBlocks);
   p.n_blocks = static_cast<int>((pb.N + BN - 1) / BN);
+  p.b_early = pb.b_const ? 1 : 0;
   p.status = device_status_word();
-  const int64_t tiles = (pb.M + BM - 1) / BM * p.n_blocks;
-  if (tiles > INT32_MAX) {
-    set_error(HOM_ERR_UNSUPPORTED, "4-bit product: more than 2^31 - 1 output tiles");
-    return false;
-  }
+  const int64_t ctas = (pb.M + BM - 1) / BM * p.n_blocks * parts;
   LaunchScope scope(kOpGemm, product_flops(pb), product_bytes(pb));
-  return check_cuda(launch_pdl(gemm_mxf4_kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kSmemBytes, stream,
-                               1, tmA, tmB, tmSA, tmSB, tmD, p),
+  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmemBytes, stream,
+                               static_cast<unsigned>(parts), tmA, tmB, tmSA, tmSB, p),
                     "4-bit product launch");
+}
+
+}  // namespace
+
+// Measured per call in a chain of calls (us):
+//   one wave of 128 x 64 tiles against the pairs' 256 x 256: 1024 x 1024 x 1024 5.5 / 5.7,
+//   1024 x 1024 x 4096 7.9 / 9.4, 512 x 2304 x 768 5.5 / 5.5; more than one wave: 512 x 4096 x 1024
+//   10.7 / 5.8, 2048 x 1024 x 1024 10.6 / 5.9;
+//   K in one, two and four parts: 64 x 1024 x 4096 6.6 / 4.8 / 4.6, 128 x 4096 x 4096 7.5 / 6.4 / 12.5
+//   (the last no longer in one wave), 128 x 1024 x 1024 5.0 / 4.6 / 4.8, 385 x 1001 x 808 9.6 / 7.5.
+bool run_product(const Problem &pb, cudaStream_t stream) {
+  if (pb.M <= kMaxFewRows) return run_product_rows(pb, stream);
+  const int64_t tiles = (pb.M + BM - 1) / BM * ((pb.N + BN - 1) / BN), sms = sm_count();
+  if (tiles > sms) return run_product_pair(pb, stream);
+  const int64_t steps = (pb.blocks + kStepBlocks - 1) / kStepBlocks;
+  // (clusters of four need SMs of one GPC: not quite all of the chip can be had)
+  const int parts = steps >= 8 && tiles * kMaxParts <= sms - sms / 8 ? kMaxParts : steps >= 4 && 2 * tiles <= sms ? 2 : 1;
+  return pb.N % 8 == 0 ? launch<true>(pb, parts, stream) : launch<false>(pb, parts, stream);
 }
 
 }  // namespace mxf4

@@ -185,47 +185,44 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales,
         make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-// x stored [cols, rows]: a thread owns one row of the result, that is one column of x, for one
-// scale tile (128 values, read 32 at a time: neighbouring threads read neighbouring elements).
+// x stored [cols, rows]: a thread owns one block of one row of the result, that is 32 values of a
+// column of x, all of them in flight; neighbouring threads read neighbouring elements.  A CTA makes
+// one scale tile, whose bytes it gathers in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kTileRows)
-quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales,
-                        long long rows, int cols, int blocks) {
+__global__ void __launch_bounds__(kTileRows * kTileBlocks)
+quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks) {
+  __shared__ __align__(16) uint8_t tile_bytes[kTileBytes];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
-  const int t = threadIdx.x;
-  const long long row = static_cast<long long>(blockIdx.x) * kTileRows + t;
-  const int tile = blockIdx.y, tile_cols = gridDim.y;
-  uint32_t word = 0;
+  const int r = threadIdx.x, b = threadIdx.y;
+  const long long row = static_cast<long long>(blockIdx.x) * kTileRows + r;
+  const int block = static_cast<int>(blockIdx.y) * kTileBlocks + b;
+  const T *from = x + static_cast<long long>(block) * kBlock * rows + row;
+  float v[kBlock];
 #pragma unroll
-  for (int b = 0; b < kTileBlocks; ++b) {
-    const int block = tile * kTileBlocks + b;
-    float v[kBlock];
+  for (int j = 0; j < kBlock; ++j)
+    v[j] = row < rows && block * kBlock + j < cols ? to_float(from[j * rows]) : 0.f;
+  uint32_t bits = 0;
 #pragma unroll
-    for (int j = 0; j < kBlock; ++j) {
-      const int c = block * kBlock + j;
-      v[j] = row < rows && c < cols ? to_float(x[c * rows + row]) : 0.f;
-    }
-    uint32_t bits = 0;
+  for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(v[j]));
+  const uint32_t byte = scale_byte(bits);
+  const float inv = reciprocal_scale(byte);
+  uint32_t packed[4];
 #pragma unroll
-    for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(v[j]));
-    const uint32_t byte = scale_byte(bits);
-    const float inv = reciprocal_scale(byte);
-    uint32_t packed[4];
+  for (int q = 0; q < 4; ++q) {
+    float part[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float part[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) part[j] = byte == 255u ? 0.f : v[q * 8 + j] * inv;
-      packed[q] = encode8(part);
-    }
-    if (row < rows && block < blocks)
-      *reinterpret_cast<uint4 *>(codes + (row * blocks + block) * 16) =
-          make_uint4(packed[0], packed[1], packed[2], packed[3]);
-    word |= byte << (8 * b);
+    for (int j = 0; j < 8; ++j) part[j] = byte == 255u ? 0.f : v[q * 8 + j] * inv;
+    packed[q] = encode8(part);
   }
-  *reinterpret_cast<uint32_t *>(scales + (static_cast<long long>(blockIdx.x) * tile_cols + tile) * kTileBytes +
-                                (t & 31) * 16 + (t >> 5) * 4) = word;
+  if (row < rows && block < blocks)
+    *reinterpret_cast<uint4 *>(codes + (row * blocks + block) * 16) =
+        make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  tile_bytes[(r & 31) * 16 + (r >> 5) * 4 + b] = static_cast<uint8_t>(byte);
+  __syncthreads();
+  if (b == 0 && r < kTileBytes / 16)
+    reinterpret_cast<uint4 *>(scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[r] =
+        reinterpret_cast<const uint4 *>(tile_bytes)[r];
 }
 
 // The way back, with the same division of work.
@@ -316,7 +313,7 @@ bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int6
     LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
     return check_cuda(launch_pdl(quantize_columns_kernel<T>,
                                  dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>(tile_cols)),
-                                 dim3(kTileRows), 0, stream, 1, x, codes, scales, rows_ll, cols_i, blocks_i),
+                                 dim3(kTileRows, kTileBlocks), 0, stream, 1, x, codes, scales, rows_ll, cols_i, blocks_i),
                       what);
   }
   const int64_t segments = (cols + kSegment - 1) / kSegment;

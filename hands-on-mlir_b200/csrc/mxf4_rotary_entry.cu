@@ -233,8 +233,8 @@ void rotary_entry(const char *name, int64_t rankX, void *dstX, int64_t rankPos, 
     set_error(HOM_ERR_INVALID, "%s: the last dimension must be contiguous", name);
     return;
   }
-  if (heads * dim > INT32_MAX) {
-    set_error(HOM_ERR_UNSUPPORTED, "%s: a token has more than 2^31 - 1 elements", name);
+  if (heads * dim > INT32_MAX || bs * seq > INT32_MAX) {
+    set_error(HOM_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens, or elements in a token", name);
     return;
   }
   if (!aligned(X.ptr, sizeof(T)) || !aligned(O.ptr, sizeof(T))) {

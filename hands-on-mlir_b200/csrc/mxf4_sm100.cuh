@@ -54,7 +54,10 @@ inline double product_bytes(const Problem &pb) {
          (pb.c_mode == 2 ? 2.0 * pb.N : 0.0);
 }
 bool run_product(const Problem &pb, cudaStream_t stream);
-// On persistent CTA pairs, 256 x 256 tiles (gemm_mxf4_pair_sm100.cu); needs N % 8 == 0.
+// For one or two rows (gemm_mxf4_rows.cu).
+constexpr int64_t kMaxFewRows = 2;
+bool run_product_rows(const Problem &pb, cudaStream_t stream);
+// On persistent CTA pairs, 256 x 256 tiles (gemm_mxf4_pair_sm100.cu).
 bool run_product_pair(const Problem &pb, cudaStream_t stream);
 
 }  // namespace mxf4

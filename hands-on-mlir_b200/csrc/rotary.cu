@@ -24,9 +24,10 @@ struct Params {
   const long long *positions;
   long long positions_b;
   const double *frequencies;
-  long long tokens;
-  int seq, heads, dim, half;
-  int chunks, heads_per_chunk;  // a warp takes one token's heads [c * heads_per_chunk, ...)
+  uint32_t tokens, seq;
+  int heads, dim, half;
+  uint32_t chunks;              // a warp takes one token's heads
+  int heads_per_chunk;          // [c * heads_per_chunk, ...)
   float magnitude, sign;
 };
 
@@ -50,50 +51,8 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ void from_float(float x, float &o) { o = x; }
 __device__ __forceinline__ void from_float(float x, __half &o) { o = __float2half_rn(x); }
 
-// One warp per token (or per token and group of heads, where there are too few tokens to fill the
-// chip).  The warp forms the token's sines and cosines once, in shared memory, and then walks over
-// its heads; a task is VEC pairs of a head, two 16-byte vectors.  The first tasks' loads are under
-// way while the sines are formed.
-template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const Params p) {
-  extern __shared__ float2 turns[];
-  hom::ptx::pdl_launch_dependents();
-  hom::ptx::pdl_wait();
-  using V = Vec<T, VEC>;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  if (unit >= p.tokens * p.chunks) return;
-  const long long token = unit / p.chunks;
-  const long long b = token / p.seq, s = token % p.seq;
-  const int head0 = static_cast<int>(unit % p.chunks) * p.heads_per_chunk;
-  const int heads = min(p.heads_per_chunk, p.heads - head0);
-  const T *x = static_cast<const T *>(p.x) + b * p.x_b + s * p.x_s + head0 * p.x_h;
-  T *out = static_cast<T *>(p.out) + b * p.out_b + s * p.out_s + head0 * p.out_h;
-  float2 *turn = turns + warp * p.half;
-
-  const int per_head = p.half / VEC;
-  const int tasks = heads * per_head;
-  V first[kBatch], second[kBatch];
-  auto place = [&](int task, int *head, int *pair) {
-    *head = task / per_head;
-    *pair = (task - *head * per_head) * VEC;
-  };
-  auto load = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int task = base + i * 32 + lane;
-      if (task < tasks) {
-        int head, pair;
-        place(task, &head, &pair);
-        const T *src = x + head * p.x_h;
-        first[i] = *reinterpret_cast<const V *>(src + (INTERLEAVED ? 2 * pair : pair));
-        second[i] = *reinterpret_cast<const V *>(src + (INTERLEAVED ? 2 * pair + VEC : p.half + pair));
-      }
-    }
-  };
-  load(0);
-
-  const long long position = p.positions ? p.positions[b * p.positions_b + s] : s;
+// The sines and cosines of one token, formed by one warp.
+__device__ __forceinline__ void form_turns(const Params &p, long long position, float2 *turn, int lane) {
   for (int i = lane; i < p.half; i += 32) {
     const double whole = static_cast<double>(position) * (p.frequencies[i] * 0.15915494309189533577);  // 1 / (2 pi)
     const float part = static_cast<float>(whole - rint(whole));
@@ -102,39 +61,133 @@ __global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const Params p) {
     turn[i] = make_float2(p.magnitude * cosine, p.magnitude * p.sign * sine);
   }
   __syncwarp();
+}
 
-  for (int base = 0; base < tasks; base += 32 * kBatch) {
-    if (base) load(base);
+// Turns VEC pairs held in two vectors: pair k is (first[k], second[k]), or, interleaved, the k-th two
+// neighbours of their sequence.
+template <typename T, int VEC, bool INTERLEAVED>
+__device__ __forceinline__ void apply_turns(Vec<T, VEC> &first, Vec<T, VEC> &second, const float2 *turn) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int task = base + i * 32 + lane;
-      if (task < tasks) {
-        int head, pair;
-        place(task, &head, &pair);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float2 t = turn[pair + k];
-          // pair k of the two vectors: (first[k], second[k]), or two neighbours of their sequence
-          T &e0 = !INTERLEAVED || VEC == 1 ? first[i].v[k] : 2 * k < VEC ? first[i].v[2 * k % VEC] : second[i].v[2 * k % VEC];
-          T &e1 = !INTERLEAVED || VEC == 1 ? second[i].v[k]
-                  : 2 * k < VEC            ? first[i].v[(2 * k + 1) % VEC]
-                                           : second[i].v[(2 * k + 1) % VEC];
-          const float x0 = to_float(e0), x1 = to_float(e1);
-          from_float(x0 * t.x - x1 * t.y, e0);
-          from_float(x1 * t.x + x0 * t.y, e1);
-        }
-        T *dst = out + head * p.out_h;
-        *reinterpret_cast<V *>(dst + (INTERLEAVED ? 2 * pair : pair)) = first[i];
-        *reinterpret_cast<V *>(dst + (INTERLEAVED ? 2 * pair + VEC : p.half + pair)) = second[i];
-      }
-    }
+  for (int k = 0; k < VEC; ++k) {
+    const float2 t = turn[k];
+    T &e0 = !INTERLEAVED || VEC == 1 ? first.v[k] : 2 * k < VEC ? first.v[2 * k % VEC] : second.v[2 * k % VEC];
+    T &e1 = !INTERLEAVED || VEC == 1 ? second.v[k] : 2 * k < VEC ? first.v[(2 * k + 1) % VEC] : second.v[(2 * k + 1) % VEC];
+    const float x0 = to_float(e0), x1 = to_float(e1);
+    from_float(x0 * t.x - x1 * t.y, e0);
+    from_float(x1 * t.x + x0 * t.y, e1);
   }
-  // the dimensions that are not turned
-  if (p.out != p.x) {
-    const int rest = (p.dim - 2 * p.half) / VEC;
-    for (int task = lane; task < heads * rest; task += 32) {
-      const int head = task / rest, d = 2 * p.half + (task - head * rest) * VEC;
-      *reinterpret_cast<V *>(out + head * p.out_h + d) = *reinterpret_cast<const V *>(x + head * p.x_h + d);
+}
+
+// One warp per token, or per token and group of heads where there are too few tokens to fill the
+// chip.  The warp forms the token's sines and cosines once, in shared memory, and walks over its
+// heads; a task is VEC pairs of a head, two 16-byte vectors, or two vectors of its other dimensions,
+// which are copied.  The first tasks' loads are under way while the sines are formed.
+//
+// FIXED: the tasks of a head are a power of two up to 32 and all turn pairs, so that a lane works on
+// the same pairs of every head and keeps their sines and cosines in registers.
+template <typename T, int VEC, bool INTERLEAVED, bool FIXED>
+__global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const Params p) {
+  extern __shared__ float2 turns[];
+  hom::ptx::pdl_launch_dependents();
+  hom::ptx::pdl_wait();
+  using V = Vec<T, VEC>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t unit = blockIdx.x * kWarps + warp;
+  const uint32_t token = unit / p.chunks;
+  if (token >= p.tokens) return;
+  const uint32_t b = token / p.seq, s = token - b * p.seq;
+  const int head0 = static_cast<int>(unit - token * p.chunks) * p.heads_per_chunk;
+  const int heads = min(p.heads_per_chunk, p.heads - head0);
+  const T *x = static_cast<const T *>(p.x) + b * p.x_b + s * p.x_s + head0 * p.x_h;
+  T *out = static_cast<T *>(p.out) + b * p.out_b + s * p.out_s + head0 * p.out_h;
+  float2 *turn = turns + warp * p.half;
+  const long long position = p.positions ? p.positions[b * p.positions_b + s] : s;
+
+  V first[kBatch], second[kBatch];
+  if constexpr (FIXED) {
+    const int per_head = p.half / VEC;  // a power of two
+    const int pair = (lane & (per_head - 1)) * VEC, at_once = 32 / per_head;
+    const int off0 = INTERLEAVED ? 2 * pair : pair, off1 = INTERLEAVED ? 2 * pair + VEC : p.half + pair;
+    int head = lane / per_head;
+    auto load = [&]() {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (head + i * at_once < heads) {
+          const T *src = x + (head + i * at_once) * p.x_h;
+          first[i] = *reinterpret_cast<const V *>(src + off0);
+          second[i] = *reinterpret_cast<const V *>(src + off1);
+        }
+      }
+    };
+    load();
+    form_turns(p, position, turn, lane);
+    float2 mine[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) mine[k] = turn[pair + k];
+    while (head < heads) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (head + i * at_once < heads) {
+          apply_turns<T, VEC, INTERLEAVED>(first[i], second[i], mine);
+          T *dst = out + (head + i * at_once) * p.out_h;
+          *reinterpret_cast<V *>(dst + off0) = first[i];
+          *reinterpret_cast<V *>(dst + off1) = second[i];
+        }
+      }
+      head += kBatch * at_once;
+      load();
+    }
+  } else {
+    // tasks of a head: its pairs, then two vectors at a time of what is copied
+    const int pairs = p.half / VEC, rest = p.out != p.x ? (p.dim - 2 * p.half) / VEC : 0;
+    const int per_head = pairs + (rest + 1) / 2;
+    const int tasks = heads * per_head;
+    const float inverse = 1.f / static_cast<float>(per_head);
+    // head and offsets of a task; the quotient by way of fp32 is off by little for a large task and
+    // put right
+    struct Place {
+      int head, pair, off0, off1;
+      bool two;
+    };
+    auto place = [&](int task) {
+      Place at;
+      at.head = static_cast<int>(static_cast<float>(task) * inverse);
+      int i = task - at.head * per_head;
+      while (i < 0) i += per_head, --at.head;
+      while (i >= per_head) i -= per_head, ++at.head;
+      at.pair = i < pairs ? i * VEC : -1;
+      at.off0 = i >= pairs ? 2 * p.half + (i - pairs) * 2 * VEC : INTERLEAVED ? 2 * i * VEC : i * VEC;
+      at.off1 = i >= pairs || INTERLEAVED ? at.off0 + VEC : p.half + i * VEC;
+      at.two = i < pairs || (i - pairs) * 2 + 1 < rest;
+      return at;
+    };
+    auto load = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int task = base + i * 32 + lane;
+        if (task < tasks) {
+          const Place at = place(task);
+          const T *src = x + at.head * p.x_h;
+          first[i] = *reinterpret_cast<const V *>(src + at.off0);
+          if (at.two) second[i] = *reinterpret_cast<const V *>(src + at.off1);
+        }
+      }
+    };
+    load(0);
+    form_turns(p, position, turn, lane);
+    for (int base = 0; base < tasks; base += 32 * kBatch) {
+      if (base) load(base);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int task = base + i * 32 + lane;
+        if (task < tasks) {
+          const Place at = place(task);
+          if (at.pair >= 0) apply_turns<T, VEC, INTERLEAVED>(first[i], second[i], turn + at.pair);
+          T *dst = out + at.head * p.out_h;
+          *reinterpret_cast<V *>(dst + at.off0) = first[i];
+          if (at.two) *reinterpret_cast<V *>(dst + at.off1) = second[i];
+        }
+      }
     }
   }
 }
@@ -167,8 +220,8 @@ bool launch(const Problem &pb, cudaStream_t stream) {
   p.positions = reinterpret_cast<const long long *>(pb.positions);
   p.positions_b = pb.positions_stride_b;
   p.frequencies = pb.frequencies;
-  p.tokens = pb.batch * pb.seq;
-  p.seq = static_cast<int>(pb.seq);
+  p.tokens = static_cast<uint32_t>(pb.batch * pb.seq);
+  p.seq = static_cast<uint32_t>(pb.seq);
   p.heads = static_cast<int>(pb.heads);
   p.dim = static_cast<int>(pb.dim);
   p.half = static_cast<int>(pb.half);
@@ -176,17 +229,17 @@ bool launch(const Problem &pb, cudaStream_t stream) {
   p.sign = pb.backward ? -1.f : 1.f;
   // Few tokens: their heads are spread over more warps, each of which forms the sines anew.
   const long long want = 16LL * sm_count();
-  long long chunks = p.tokens >= want ? 1 : (want + p.tokens - 1) / p.tokens;
+  const long long tokens = p.tokens;
+  long long chunks = tokens >= want ? 1 : (want + tokens - 1) / tokens;
   if (chunks > p.heads) chunks = p.heads;
   p.heads_per_chunk = static_cast<int>((p.heads + chunks - 1) / chunks);
-  p.chunks = (p.heads + p.heads_per_chunk - 1) / p.heads_per_chunk;
-  const long long grid = (p.tokens * p.chunks + kWarps - 1) / kWarps;
-  if (grid > INT32_MAX) {
-    set_error(HOM_ERR_UNSUPPORTED, "rotary positions: more than 2^31 - 1 thread blocks");
-    return false;
-  }
-  auto kernel = pb.interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>;
-  const double elements = static_cast<double>(p.tokens) * p.heads * p.dim;
+  p.chunks = static_cast<uint32_t>((p.heads + p.heads_per_chunk - 1) / p.heads_per_chunk);
+  const long long grid = (static_cast<long long>(p.tokens) * p.chunks + kWarps - 1) / kWarps;
+  const int per_head = p.half / VEC;
+  const bool fixed = per_head <= 32 && (per_head & (per_head - 1)) == 0 && (p.dim == 2 * p.half || p.out == p.x);
+  auto kernel = pb.interleaved ? (fixed ? rotary_kernel<T, VEC, true, true> : rotary_kernel<T, VEC, true, false>)
+                               : (fixed ? rotary_kernel<T, VEC, false, true> : rotary_kernel<T, VEC, false, false>);
+  const double elements = static_cast<double>(pb.batch) * pb.seq * pb.heads * pb.dim;
   LaunchScope scope(kOpRotary, 0.0, 2.0 * sizeof(T) * elements);
   return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps),
                                kWarps * p.half * sizeof(float2), stream, 1, p),

@@ -332,7 +332,8 @@ HOM_EXPORT void homGemmMxF4F16(int64_t rankA, void *dstA, int64_t rankSA, void *
  * beyond 2F are copied.  X, Out [bs, seq, heads, d] with any non-negative strides and a contiguous
  * last dimension - the query and key heads of a packed [bs, seq, 3*heads*d] are the view
  * [bs, seq, 2*heads, d] of it -; Out may be X, otherwise they must not overlap.  Positions int64
- * [bs, seq] or [1, seq], absent (rank 0 / null): 0 .. seq - 1.  Frequencies fp64 [F], F <= 512;
+ * [bs, seq] or [1, seq], absent (rank 0 / null): 0 .. seq - 1; bs * seq and heads * d below 2^31.
+ * Frequencies fp64 [F], F <= 512;
  * angles are formed in 64 bits, so that far positions keep their fractions of a turn.  The
  * rotation is fp32, rounded once.
  * No counterpart in the reference, whose model adds a position table. */
