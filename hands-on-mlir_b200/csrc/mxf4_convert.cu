@@ -78,16 +78,6 @@ __device__ __forceinline__ void decode8(uint32_t codes, float (&v)[8]) {
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-__device__ __forceinline__ void load8(const __half *p, float (&v)[8]) {
-  const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-  const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(h[j]);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
-  }
-}
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
   const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
@@ -107,71 +97,127 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 __device__ __forceinline__ void store1(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store1(float *p, float v) { *p = v; }
 
+// Eight consecutive values of a row as they lie in memory, the bits of their largest magnitude as
+// fp32 (NaN and infinity above all numbers), and their codes.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<__half> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const __half *p) { raw = *reinterpret_cast<const uint4 *>(p); }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    __half2 *h = reinterpret_cast<__half2 *>(&raw);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  }
+  __device__ __forceinline__ void clear() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t largest() const {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return magnitude_bits(__half2float(__hmax_nan(__low2half(m), __high2half(m))));
+  }
+  __device__ __forceinline__ uint32_t encode(float inv) const {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(h[j]);
+      v[2 * j] = f.x * inv;
+      v[2 * j + 1] = f.y * inv;
+    }
+    return encode8(v);
+  }
+};
+template <>
+struct Eight<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float *p) { load8(p, v); }
+  __device__ __forceinline__ void set(const float (&w)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = w[j];
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  }
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits = max(bits, magnitude_bits(v[j]));
+    return bits;
+  }
+  __device__ __forceinline__ uint32_t encode(float inv) const {
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = v[j] * inv;
+    return encode8(s);
+  }
+};
+
 // One warp converts a segment of 256 columns of the rows r, r + 32, r + 64 and r + 96 of a
 // 128-row group: four independent loads in flight, and the scales of the four rows are the 16
-// consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED:
-// rows start on 16 bytes (cols % 8 == 0); otherwise the warp reads element by element, coalesced,
-// and sorts the values through shared memory.
+// consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED: rows
+// start on 16 bytes (cols % 8 == 0); otherwise the warp reads element by element, coalesced, and
+// sorts the values through shared memory.  (A persistent form that requests the next unit's values
+// early was slower: its registers cost more loads in flight than it gains.)
+//
+// What the rows kernel needs is many loads in flight, so its registers are held down: 65536 x 4096
+// fp16 values 119 us with room for five CTAs on an SM, 112 for eight (6.0 TB/s); 20011 x 776 fp32
+// values 13.0 with five, 13.5 with six, 26 (spills) with eight.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps)
-quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales,
-                     long long rows, int cols, int blocks, int segments, long long units) {
-  __shared__ float sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 4 : kSegment];
+__global__ void __launch_bounds__(32 * kWarps, sizeof(T) == 2 && ALIGNED ? 8 : 5)
+quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks,
+                     uint32_t segments, long long units) {
+  __shared__ __align__(16) T sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 8 : kSegment];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
   if (unit >= units) return;
-  const long long group = unit / segments / kRowStep;
-  const int segment = static_cast<int>(unit % segments);
-  const int r = static_cast<int>(unit / segments % kRowStep);
+  const long long row_unit = units <= INT32_MAX ? static_cast<uint32_t>(unit) / segments : unit / segments;
+  const int segment = static_cast<int>(unit - row_unit * segments);
+  const long long group = row_unit / kRowStep;
+  const int r = static_cast<int>(row_unit % kRowStep);
   const long long row0 = group * kTileRows + r;
   const int col = segment * kSegment + lane * kLaneValues;
 
-  float v[4][8];
+  Eight<T> v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const long long row = row0 + i * kRowStep;
     if (ALIGNED) {
-      if (row < rows && col < cols) {
-        load8(x + row * cols + col, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      }
+      if (row < rows && col < cols) v[i].load(x + row * cols + col);
+      else v[i].clear();
     } else {
+      float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int c = segment * kSegment + j * 32 + lane;
-        v[i][j] = row < rows && c < cols ? to_float(x[row * cols + c]) : 0.f;
+        w[j] = row < rows && c < cols ? to_float(x[row * cols + c]) : 0.f;
       }
-    }
-  }
-  if (!ALIGNED) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sorted[warp][j * 32 + lane] = v[i][j];
-      __syncwarp();
-      load8(&sorted[warp][lane * kLaneValues], v[i]);
-      __syncwarp();
+      v[i].set(w);
     }
   }
   uint32_t words[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t bits = 0;
+    if (!ALIGNED) {
+      // value j * 32 + lane of the segment in slot j of the lane -> eight consecutive ones
+      const T *mine = reinterpret_cast<const T *>(&v[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bits = max(bits, magnitude_bits(v[i][j]));
+      for (int j = 0; j < 8; ++j) sorted[warp][j * 32 + lane] = mine[j];
+      __syncwarp();
+      v[i].load(&sorted[warp][lane * kLaneValues]);
+      __syncwarp();
+    }
+    uint32_t bits = v[i].largest();
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
     const uint32_t byte = scale_byte(bits);
-    const float inv = reciprocal_scale(byte);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = byte == 255u ? 0.f : v[i][j] * inv;
+    const uint32_t packed = byte == 255u ? 0u : v[i].encode(reciprocal_scale(byte));
     const long long row = row0 + i * kRowStep;
     if (row < rows && col < blocks * kBlock)
-      *reinterpret_cast<uint32_t *>(codes + row * (blocks * 16LL) + col / 2) = encode8(v[i]);
+      *reinterpret_cast<uint32_t *>(codes + row * (blocks * 16LL) + col / 2) = packed;
     // the bytes of four neighbouring blocks become the word of one scale tile
     uint32_t word = byte << (8 * ((lane >> 2) & 3));
     word |= __shfl_xor_sync(0xffffffffu, word, 4);
@@ -185,44 +231,59 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales,
         make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-// x stored [cols, rows]: a thread owns one block of one row of the result, that is 32 values of a
-// column of x, all of them in flight; neighbouring threads read neighbouring elements.  A CTA makes
-// one scale tile, whose bytes it gathers in shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kTileRows * kTileBlocks)
+// x stored [cols, rows]: a thread owns one block of COLUMNS rows of the result, that is 32 values of
+// as many columns of x, all of them in flight; neighbouring threads read neighbouring elements.  A
+// CTA makes one scale tile, whose bytes it gathers in shared memory.  Two columns for fp16 (rows even,
+// x on 4 bytes): with 2-byte loads a 4096 x 4096 weight took 27.7 us.
+template <typename T, int COLUMNS>
+__global__ void __launch_bounds__(kTileRows * kTileBlocks / COLUMNS)
 quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks) {
   __shared__ __align__(16) uint8_t tile_bytes[kTileBytes];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
-  const int r = threadIdx.x, b = threadIdx.y;
-  const long long row = static_cast<long long>(blockIdx.x) * kTileRows + r;
+  struct __align__(sizeof(T) * COLUMNS) Few {
+    T v[COLUMNS];
+  };
+  const int r0 = static_cast<int>(threadIdx.x) * COLUMNS, b = threadIdx.y;
+  const long long row0 = static_cast<long long>(blockIdx.x) * kTileRows + r0;
   const int block = static_cast<int>(blockIdx.y) * kTileBlocks + b;
-  const T *from = x + static_cast<long long>(block) * kBlock * rows + row;
-  float v[kBlock];
+  const T *from = x + static_cast<long long>(block) * kBlock * rows + row0;
+  Few v[kBlock];
 #pragma unroll
-  for (int j = 0; j < kBlock; ++j)
-    v[j] = row < rows && block * kBlock + j < cols ? to_float(from[j * rows]) : 0.f;
-  uint32_t bits = 0;
+  for (int j = 0; j < kBlock; ++j) {
+    if (row0 < rows && block * kBlock + j < cols) {
+      v[j] = *reinterpret_cast<const Few *>(from + j * rows);
+    } else {
 #pragma unroll
-  for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(v[j]));
-  const uint32_t byte = scale_byte(bits);
-  const float inv = reciprocal_scale(byte);
-  uint32_t packed[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    float part[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) part[j] = byte == 255u ? 0.f : v[q * 8 + j] * inv;
-    packed[q] = encode8(part);
+      for (int c = 0; c < COLUMNS; ++c) v[j].v[c] = T(0.f);
+    }
   }
-  if (row < rows && block < blocks)
-    *reinterpret_cast<uint4 *>(codes + (row * blocks + block) * 16) =
-        make_uint4(packed[0], packed[1], packed[2], packed[3]);
-  tile_bytes[(r & 31) * 16 + (r >> 5) * 4 + b] = static_cast<uint8_t>(byte);
+#pragma unroll
+  for (int c = 0; c < COLUMNS; ++c) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(to_float(v[j].v[c])));
+    const uint32_t byte = scale_byte(bits);
+    const float inv = reciprocal_scale(byte);
+    uint32_t packed[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float part[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[j] = to_float(v[q * 8 + j].v[c]) * inv;
+      packed[q] = byte == 255u ? 0u : encode8(part);
+    }
+    if (row0 < rows && block < blocks)
+      *reinterpret_cast<uint4 *>(codes + ((row0 + c) * blocks + block) * 16) =
+          make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    const int r = r0 + c;
+    tile_bytes[(r & 31) * 16 + (r >> 5) * 4 + b] = static_cast<uint8_t>(byte);
+  }
   __syncthreads();
-  if (b == 0 && r < kTileBytes / 16)
-    reinterpret_cast<uint4 *>(scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[r] =
-        reinterpret_cast<const uint4 *>(tile_bytes)[r];
+  const int t = static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x);
+  if (t < kTileBytes / 16)
+    reinterpret_cast<uint4 *>(scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[t] =
+        reinterpret_cast<const uint4 *>(tile_bytes)[t];
 }
 
 // The way back, with the same division of work.
@@ -311,9 +372,12 @@ bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int6
       return false;
     }
     LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
-    return check_cuda(launch_pdl(quantize_columns_kernel<T>,
+    constexpr int kColumns = sizeof(T) == 2 ? 2 : 1;
+    const bool two = kColumns == 2 && rows % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & 3u) == 0;
+    return check_cuda(launch_pdl(two ? quantize_columns_kernel<T, kColumns> : quantize_columns_kernel<T, 1>,
                                  dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>(tile_cols)),
-                                 dim3(kTileRows, kTileBlocks), 0, stream, 1, x, codes, scales, rows_ll, cols_i, blocks_i),
+                                 dim3(kTileRows / (two ? 2 : 1), kTileBlocks), 0, stream, 1, x, codes, scales, rows_ll,
+                                 cols_i, blocks_i),
                       what);
   }
   const int64_t segments = (cols + kSegment - 1) / kSegment;
@@ -323,7 +387,7 @@ bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int6
   auto kernel = cols % kLaneValues == 0 && is_aligned16(x) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
   LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
   return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, x, codes,
-                               scales, rows_ll, cols_i, blocks_i, static_cast<int>(segments), units),
+                               scales, rows_ll, cols_i, blocks_i, static_cast<uint32_t>(segments), units),
                     what);
 }
 
