@@ -5,19 +5,19 @@
 // 128 rows of B and the accumulator of its 128 output rows.  The grid is persistent.  A step is 256
 // values along K; its four 256 x 256 x 64 MMAs take 512 tensor-pipe cycles.
 //
-// What comes to an SM per step of a tile is 35 KB in 512 cycles, near what L2 delivers (13 to 15
-// TB/s here).  With up to four steps (K <= 1024) A's rows can stay in shared memory while the pair
-// works through the column tiles of a row block ("resident"), and only B streams.  Products with
-// small K are bound by writing D: 32768 x 4096 x 1024 takes 70 us, a plain fill of D 68.
+// What bounds it: a step brings 35 KB to each SM, and with four stages in flight L2 delivers some
+// 16 TB/s.  Timed by leaving parts out, 16384 x 4096 x 4096 (107 us) takes 77 us with a quarter of
+// the MMAs and no stores, 74 with neither loads nor stores: the two overlap, but not wholly.  The
+// scale copies cost 5 %.  With up to four steps (K <= 1024) A's rows can stay in shared memory while
+// the pair works through the column tiles of a row block ("resident"), and only B streams.
 //
-// Tensor memory: the two accumulators share 64 columns - the first lies in [0, 256), the second in
-// [192, 448) - because the scales need 2 x 24 columns behind them.  The warps that drain the shared
-// columns take all 64 into registers at once, so that the next tile's MMAs can start while the
-// other three quarters are drained beside them.  (192-column tiles, whose accumulators need not
-// share, were slower at every size: they pull 13 % more through L2 for the same work.)
-//
-// A set of scales is written for step i + 2 only when the MMAs of step i have completed: copies
-// are ordered before later MMAs of the thread, but not behind earlier ones.
+// Tensor memory: every stage of the ring has its own 24 columns of scales, so that the issuing
+// thread waits for nothing but the stage: that it was filled again says that the MMAs of its last
+// use, and their reads of the scales, are over.  Two whole accumulators do not fit beside 96 columns
+// of scales: the first lies in [0, 256), the second in [160, 416), and the warps that drain the 96
+// columns they share take them into registers at once, so that the next tile's MMAs can start while
+// the rest is drained beside them.  (192-column tiles need not share, but pull 13 % more through L2
+// for the same work: 16384 x 4096 x 4096 120 us, 32768 x 4096 x 1024 73 instead of 69.)
 //
 //   warps 0, 2, 3  TMA producers of A's codes, of B's and of the scales
 //   warp 1         tensor memory, scale copies and MMA issue (even CTA)
@@ -44,25 +44,26 @@ constexpr int kStepTiles = kStepBlocks / kTileBlocks;  // 2 scale tiles along K
 constexpr int kStages = 4;                             // and the steps that A may have to stay resident
 constexpr int kControlWarps = 4;
 constexpr int kMaxPairs = 512;                         // of any device, generously
-constexpr int kDrainWarps = 16;
-constexpr int kThreads = 32 * (kControlWarps + kDrainWarps);
 constexpr uint32_t kCodeBytes = kHalf * kStepBytes;    // of one operand, per CTA and stage
 constexpr uint32_t kScaleABytes = kStepTiles * kTileBytes, kScaleBBytes = 2 * kScaleABytes;
-constexpr uint32_t kAStageBytes = kCodeBytes + kScaleABytes, kBStageBytes = kCodeBytes + kScaleBBytes;
-// tensor memory columns
-constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kSecondAcc = 192;
-constexpr uint32_t kScales = kSecondAcc + BN, kScaleSet = 4 * kStepTiles * 3, kScalesB = 4 * kStepTiles;
-
+constexpr uint32_t kAStageBytes = kCodeBytes + kScaleABytes;
+constexpr uint32_t kBStageBytes = kCodeBytes + kScaleBBytes;
+constexpr int kDrainWarps = 16;
+constexpr int kThreads = 32 * (kControlWarps + kDrainWarps);
 // shared-memory offsets: stages of A, of B, staging tiles and rows of C per epilogue warp, barriers
 constexpr uint32_t kB = kStages * kAStageBytes;
 constexpr uint32_t kStaging = kB + kStages * kBStageBytes;
 constexpr uint32_t kBias = kStaging + kDrainWarps * gemm::kEpilogueStageBytes;
-constexpr uint32_t kBars = kBias + kDrainWarps * 128;
+constexpr uint32_t kBars = kBias + kDrainWarps * 256;
 constexpr int kBarriers = 4 * kStages + 5 + kDrainWarps;
 constexpr uint32_t kSmemBytes = kBars + 8 * kBarriers + 16 + 1024;
+// tensor-memory columns
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kSecondAcc = 160, kScales = kSecondAcc + BN;
+constexpr int kSharingGroups = 2;  // 64-column groups with shared columns: the first accumulator's last, the second's first
+constexpr uint32_t kScaleSet = 4 * kStepTiles * 3, kScalesB = 4 * kStepTiles;
 static_assert(kAStageBytes % 1024 == 0 && kBStageBytes % 1024 == 0, "swizzled tiles start on 1024 bytes");
-static_assert(kScales + 2 * kScaleSet <= kTmemCols, "accumulators and scales exceed tensor memory");
+static_assert(kScales + kStages * kScaleSet <= kTmemCols, "accumulators and scales exceed tensor memory");
 static_assert(kSmemBytes <= 227 * 1024, "exceeds a CTA's shared memory");
 
 struct Params {
@@ -124,7 +125,8 @@ __device__ __forceinline__ void ragged_store(__half *d, int m, int n, int row0, 
 }
 
 // Applies the epilogue to 32 accumulators of this lane's row and leaves the fp16 results in the
-// staging tile, whose row holds C's values where C is a matrix; `bias` is the row of C otherwise.
+// staging tile, whose row holds C's values where C is a matrix; `bias` is
+// the row of C otherwise, in fp32 (in the general forms, which are short of registers, in fp16).
 template <int FORM>
 __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&acc)[32], int half, uint32_t my_row,
                                             uint32_t bias, int lane) {
@@ -134,13 +136,22 @@ __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&ac
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const uint32_t addr = my_row + ((static_cast<uint32_t>(half * 4 + g) ^ (lane & 7u)) << 4);
-    uint32_t c[4] = {0, 0, 0, 0};
-    if (full || row) {
-      const uint32_t from = row ? bias + (half * 4 + g) * 16 : addr;
+    float2 c[4];
+    if (full || (row && general(FORM))) {
+      uint32_t h[4];
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-                   : "r"(from)
+                   : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+                   : "r"(full ? addr : bias + (half * 4 + g) * 16)
                    : "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+    } else if (row) {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(c[j].x), "=f"(c[j].y), "=f"(c[j + 1].x), "=f"(c[j + 1].y)
+                     : "r"(bias + (half * 32 + g * 8 + j * 2) * 4)
+                     : "memory");
     }
     uint32_t w[4];
 #pragma unroll
@@ -149,8 +160,7 @@ __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&ac
       float2 v = make_float2(__uint_as_float(acc[i]), __uint_as_float(acc[i + 1]));
       if (general(FORM)) v = __fmul2_rn(alpha2, v);
       if (full || row) {
-        const float2 cf = __half22float2(*reinterpret_cast<const __half2 *>(&c[j]));
-        v = general(FORM) ? __ffma2_rn(beta2, cf, v) : __fadd2_rn(cf, v);
+        v = general(FORM) ? __ffma2_rn(beta2, c[j], v) : __fadd2_rn(c[j], v);
       }
       if (general(FORM) ? p.act == 1 : (FORM & kGelu) != 0) v = gelu2(v);
       const __half2 h = __floats2half2_rn(v.x, v.y);
@@ -209,7 +219,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       mbar_init(acc_full_bar(a), 1);
       mbar_init(acc_empty_bar(a), 2 * kDrainWarps);
     }
-    mbar_init(shared_bar, 2 * 4);
+    mbar_init(shared_bar, 2 * 4 * kSharingGroups);
     for (int w = 0; w < kDrainWarps; ++w) mbar_init(c_bar(w), 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -295,25 +305,20 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     if (rank == 0 && elect_one()) {
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
-      uint32_t step = 0;  // over all tiles
       int it = 0;
       for (int tile = first; tile < last && ok; tile += stride, ++it) {
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + (acc ? kSecondAcc : 0);
         const bool new_a = resident && (tile == first || tile % p.n_blocks == 0);
         const bool ends_a = resident && (tile + 1 == last || (tile + 1) % p.n_blocks == 0);
-        for (int i = 0; i < p.steps; ++i, ++step) {
-          // the MMAs that read this set of scales two steps ago have completed
-          if (step >= 2)
-            ok = mbar_wait(empty_bar((step - 2) % kStages), ((step - 2) / kStages) & 1, abort_flag, p.status,
-                           kDevWaitTimeoutMma);
-          if (ok) ok = mbar_wait(full_bar(slot), ph, abort_flag, p.status, kDevWaitTimeoutMma);
+        for (int i = 0; i < p.steps; ++i) {
+          ok = mbar_wait(full_bar(slot), ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (ok && new_a) ok = mbar_wait(a_full_bar(i), a_ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (!ok) break;
           tc_fence_after_sync();
           const uint32_t src_a = smem_base + (resident ? i : slot) * kAStageBytes;
           const uint32_t src_b = smem_base + kB + slot * kBStageBytes;
-          const uint32_t scales = tmem_base + kScales + (step & 1) * kScaleSet;
+          const uint32_t scales = tmem_base + kScales + slot * kScaleSet;
 #pragma unroll
           for (int k = 0; k < kStepTiles; ++k) {
             tc_copy_scales_pair(scales + 4 * k, make_smem_desc_scales(src_a + kCodeBytes + k * kTileBytes));
@@ -355,7 +360,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const int group = drain >> 2;
     const uint32_t stage_smem = smem_base + kStaging + drain * gemm::kEpilogueStageBytes;
     const uint32_t my_row = stage_smem + lane * 128;
-    const uint32_t bias = smem_base + kBias + drain * 128;
+    const uint32_t bias = smem_base + kBias + drain * 256;
     const bool full = general(FORM) ? p.c_mode == 1 : (FORM & kFull) != 0;
     const bool row = general(FORM) ? p.c_mode == 2 : (FORM & kRow) != 0;
     constexpr bool ragged = FORM == kRagged;
@@ -395,7 +400,12 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
       if (row) {
         __syncwarp();
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "r"(next_row) : "memory");
+        if (general(FORM)) {
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "r"(next_row) : "memory");
+        } else {
+          const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&next_row));
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(bias + 8 * lane), "f"(two.x), "f"(two.y) : "memory");
+        }
         __syncwarp();
         if (tile + stride < last) next_row = load_row(tile + stride);
       }
@@ -417,9 +427,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           ok = __all_sync(0xffffffffu, mbar_wait(c_bar(drain), it & 1, abort_flag, p.status, kDevWaitTimeoutEpilogue));
         }
       };
-      // the columns that the other accumulator shares: the first one's last group, the second one's first
-      const bool shares = group == (acc ? 0 : 3);
-      if (shares) {
+      if (acc ? group < kSharingGroups : group >= 4 - kSharingGroups) {
         uint32_t lo[32], hi[32];
         tmem_ld_32x32(t_row, lo);
         tmem_ld_32x32(t_row + 32, hi);
@@ -544,10 +552,11 @@ bool run_product_pair(const Problem &pb, cudaStream_t stream) {
   p.tiles = static_cast<int>(tiles);
   if (p.tiles < pairs) pairs = p.tiles;
   // Keeping A saves half of what is pulled through L2, but lets the pairs drift apart; measured with
-  // and without, in us: 32768 x 4096 x 1024 69.7 / 75.7, the same with GELU and a row of C (131072
-  // rows) 358 / 369, 32768 x 2304 x 768 39.6 / 40.8; with a matrix C, whose tiles are read as well,
-  // 16384 x 4096 x 1024 54.4 / 53.4, 32768 x 1024 x 1024 30.6 / 29.3, 32768 x 768 x 768 25.6 / 24.4.
+  // and without, in us: 32768 x 4096 x 1024 68 / 74, 131072 x 4096 x 1024 with GELU and a row of C
+  // 343 / 352, 32768 x 2304 x 768 38.8 / 40.6; with a matrix C, whose tiles are read as well,
+  // 16384 x 4096 x 1024 54.5 / 53.1, 32768 x 1024 x 1024 31.0 / 29.6, 32768 x 768 x 768 25.8 / 24.3.
   p.resident = p.steps <= kStages && p.tiles >= 2 * pairs && pb.c_mode != 1 ? 1 : 0;
+
   cfg.gridDim = dim3(2 * pairs);
   LaunchScope scope(kOpGemm, product_flops(pb), product_bytes(pb));
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmSA, tmSB, tmC, tmD, p),
