@@ -175,6 +175,10 @@ for _op in ("Add", "Sub", "Mul", "Div"):
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))
 
 
+#: names of homRotaryFrequencies' scalings, in the order of their numbers
+ROTARY_SCALINGS = ("none", "linear", "base", "parts")
+
+
 def mxf4_shapes(rows: int, cols: int) -> tuple[tuple[int, int], tuple[int, int, int]]:
     """Shapes of the codes and the scales (both uint8) of a [rows, cols] matrix in microscaled 4-bit
     floating point; see include/hom_nvgpu_runner_utils.h."""
@@ -329,8 +333,8 @@ class RunnerUtils:
 
     def homRotaryFrequencies(self, Out, base=10000.0, scaling="none", factor=1.0, original_length=0.0,
                              beta_fast=32.0, beta_slow=1.0):
-        """`scaling`: "none", "linear", "base" or "parts"."""
-        kind = ("none", "linear", "base", "parts").index(scaling)
+        """`scaling`: one of ROTARY_SCALINGS."""
+        kind = ROTARY_SCALINGS.index(scaling)
         self.lib.homRotaryFrequencies(*_as_args(Out), base, kind, factor, original_length, beta_fast, beta_slow)
         self.check()
 

@@ -6,10 +6,10 @@ hands it weights and inputs, and exposes the batch-sharding helpers the multi-GP
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int32, c_int64, c_void_p
 from dataclasses import dataclass
 
-from . import REPLAY_LIB, HomError, MemRef, UnrankedMemRef, runner
+from . import REPLAY_LIB, ROTARY_SCALINGS, HomError, MemRef, UnrankedMemRef, runner
 
 
 class _Config(ctypes.Structure):
@@ -91,6 +91,10 @@ def _replay_lib():
         lib.homBertSetWeight.argtypes = [c_void_p, c_int32, c_int64, c_void_p]
         lib.homBertLoadConstants.restype = c_int
         lib.homBertLoadConstants.argtypes = [c_void_p, c_int32]
+        lib.homBertQuantizeWeights.restype = c_int
+        lib.homBertQuantizeWeights.argtypes = [c_void_p]
+        lib.homBertSetRotary.restype = c_int
+        lib.homBertSetRotary.argtypes = [c_void_p, c_double, c_int32] + [c_double] * 4 + [c_float]
         lib.homBertForward.restype = c_int
         lib.homBertForward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                        c_void_p, ctypes.POINTER(UnrankedMemRef), c_int]
@@ -154,6 +158,19 @@ class BertProgram:
 
     def load_constants(self, first_idx: int = 0):
         self._rc(self._lib.homBertLoadConstants(self._handle, first_idx))
+
+    def quantize_weights(self):
+        """Run the projections in microscaled 4-bit floating point from now on, with the weights bound
+        now; call it again after binding others."""
+        self._rc(self._lib.homBertQuantizeWeights(self._handle))
+
+    def set_rotary(self, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                   original_length: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                   magnitude: float = 1.0):
+        """Turn queries and keys by their positions from now on (a model without a position table
+        binds zeros); arguments as RunnerUtils.homRotaryFrequencies."""
+        self._rc(self._lib.homBertSetRotary(self._handle, base, ROTARY_SCALINGS.index(scaling), factor, original_length,
+                                            beta_fast, beta_slow, magnitude))
 
     def forward(self, ids, mask, types, use_graph: bool = False) -> MemRef:
         """Enqueue one forward on device tensors (int64 [batch, seq]); returns the memref of

@@ -51,9 +51,20 @@ Tensor make_view(void *data, std::initializer_list<int64_t> sizes) {
   return t;
 }
 
+// A matrix in microscaled 4-bit floating point.
+struct Coded {
+  Tensor codes, scales;
+};
+
 struct Program {
   HomBertConfig cfg{};
   std::vector<Tensor> weights;
+  std::vector<Coded> coded;    // the projections in 4 bits, four per layer; empty: fp16
+  bool coded_stale = false;    // other weights were bound since
+  Coded coded_hidden, coded_ffn;  // the activations that the next product reads
+  Tensor frequencies;          // of the rotary positions; none: no rotation
+  Tensor rotated;              // the query and key heads of qkv
+  float rotary_magnitude = 1.f;
   Tensor x, type_rows, qkv, ctx, ffn, cu;  // activations (hoisted allocations)
   Tensor stats[2];  // fused_layernorm == 2: fp32 row partial sums of the raw hidden states (ping-pong)
   Tensor ids_dev, mask_dev, types_dev;     // staging for the host entry point
@@ -92,6 +103,58 @@ void release(Tensor &t, bool f16) {
 
 int status() { return homGetLastError(); }
 
+void release(Coded &c) {
+  release(c.codes, false);
+  release(c.scales, false);
+}
+
+// `shape` carved from a fresh device allocation of whole 32-bit words.
+Tensor make_bytes(std::initializer_list<int64_t> shape) {
+  int64_t bytes = 1;
+  for (int64_t s : shape) bytes *= s;
+  if (bytes / 4 >= INT32_MAX) return Tensor{};
+  HomUnrankedMemRef words = alloc1DMemRefNVGPUI32(static_cast<int32_t>((bytes + 3) / 4));
+  if (!words.descriptor) return Tensor{};
+  Tensor t = make_view(static_cast<void **>(words.descriptor)[1], shape);
+  t.owned_buffer = true;
+  std::free(words.descriptor);
+  return t;
+}
+
+bool make_coded(int64_t rows, int64_t cols, Coded *out) {
+  const int64_t blocks = (cols + 31) / 32;
+  out->codes = make_bytes({rows, 16 * blocks});
+  out->scales = make_bytes({(rows + 127) / 128, (blocks + 3) / 4, 512});
+  return out->codes.data() && out->scales.data();
+}
+
+void declare(Tensor &t) {
+  const int64_t *w = static_cast<const int64_t *>(t.desc);
+  int64_t n = 1;
+  for (int64_t i = 0; i < t.rank; ++i) n *= w[3 + i];
+  homDeclareWeights(t.data(), n);
+  t.declared = t.data();
+}
+
+// Every weight is bound, and what was quantised is of the weights bound now.
+bool ready(const Program &p) {
+  for (const Tensor &w : p.weights)
+    if (!w.desc) return false;
+  return p.coded.empty() || !p.coded_stale;
+}
+
+// What was captured no longer says what the program does; the next call runs eagerly again.
+void forget_graphs(Program &p) {
+  if (p.graph_exec) cudaGraphExecDestroy(p.graph_exec);
+  p.graph_exec = nullptr;
+  for (cudaGraphExec_t &g : p.host_graph) {
+    if (g) cudaGraphExecDestroy(g);
+    g = nullptr;
+  }
+  p.warmed_up = false;
+  p.warm_stream_valid = false;
+}
+
 // Staging kernels of the host entry point.  Copy-engine nodes between kernel nodes cost a
 // hand-over of tens of microseconds each inside a graph; plain kernels do not.
 // Reads the three int64 [batch, seq] planes straight from pinned (device-accessible) host
@@ -128,12 +191,33 @@ int issue_forward(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void
   const HomBertConfig &c = p.cfg;
   const float scale = 1.0f / std::sqrt(static_cast<float>(c.hidden / c.heads));
   auto gemm = [&](Tensor &a, Tensor &w, Tensor &cmat, Tensor &d, int64_t act, float beta) {
+    if (!p.coded.empty()) {
+      Coded &weight = p.coded[static_cast<size_t>(&w - &p.weights[3])];
+      Coded &x = &a == &p.ffn ? p.coded_ffn : p.coded_hidden;
+      // (the activations and D as matrices of batch * seq rows; C is D or not read)
+      int64_t rows[7], out[7];
+      const int64_t *from = static_cast<const int64_t *>(a.desc), *to = static_cast<const int64_t *>(d.desc);
+      for (int64_t *m : {rows, out}) {
+        const int64_t *t = m == rows ? from : to;
+        m[0] = t[0], m[1] = t[1], m[2] = t[2];
+        m[3] = t[3] * t[4], m[4] = t[5], m[5] = t[5], m[6] = 1;
+      }
+      homQuantizeMxF4F16(2, rows, false, x.codes.rank, x.codes.desc, x.scales.rank, x.scales.desc);
+      homGemmMxF4F16(x.codes.rank, x.codes.desc, x.scales.rank, x.scales.desc, weight.codes.rank, weight.codes.desc,
+                     weight.scales.rank, weight.scales.desc, 2, out, 2, out, act, 1.0f, beta);
+      return;
+    }
     if (c.weights_nk)
       nvteGemmF16(a.rank, a.desc, false, w.rank, w.desc, true, cmat.rank, cmat.desc, d.rank, d.desc,
                   act, 1.0f, beta, 0, 0);
     else
       cutlassGemmF16(a.rank, a.desc, false, w.rank, w.desc, false, cmat.rank, cmat.desc, d.rank,
                      d.desc, act, 1.0f, beta, 0, 1);
+  };
+  auto rotate = [&]() {
+    if (p.frequencies.desc)
+      homRotaryF16(p.rotated.rank, p.rotated.desc, 0, nullptr, p.frequencies.rank, p.frequencies.desc, p.rotated.rank,
+                   p.rotated.desc, false, false, p.rotary_magnitude);
   };
   thrustCuSeqLenI64(rankMask, mask, p.cu.rank, p.cu.desc);
   if (c.fused_embedding) {
@@ -168,6 +252,7 @@ int issue_forward(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void
       Tensor &w1 = p.weights[5 + 4 * l], &w2 = p.weights[6 + 4 * l];
       Tensor &s_in = cur < 0 ? none : p.stats[cur];
       deferred(p.x, s_in, wqkv, none, none, p.qkv, none, 0);
+      rotate();
       nvteBertAttentionF16(p.qkv.rank, p.qkv.desc, p.cu.rank, p.cu.desc, p.ctx.rank, p.ctx.desc, scale,
                            c.heads);
       const int mid = cur < 0 ? 0 : cur ^ 1;
@@ -183,6 +268,7 @@ int issue_forward(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void
     Tensor &wqkv = p.weights[3 + 4 * l], &wo = p.weights[4 + 4 * l];
     Tensor &w1 = p.weights[5 + 4 * l], &w2 = p.weights[6 + 4 * l];
     gemm(p.x, wqkv, p.qkv, p.qkv, 0, 0.0f);
+    rotate();
     nvteBertAttentionF16(p.qkv.rank, p.qkv.desc, p.cu.rank, p.cu.desc, p.ctx.rank, p.ctx.desc, scale,
                          c.heads);
     if (c.fused_layernorm) {
@@ -204,8 +290,7 @@ int issue_forward(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void
 
 int forward_impl(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void *mask,
                  int64_t rankTypes, void *types, int use_graph) {
-  for (const Tensor &w : p.weights)
-    if (!w.desc) return HOM_ERR_INVALID;
+  if (!ready(p)) return HOM_ERR_INVALID;
   if (!use_graph || !p.warmed_up) {
     // The first call always runs eagerly: it performs the library's one-time set-up
     // (kernel attributes, tensor-map cache), which must not happen during capture.
@@ -327,6 +412,11 @@ void homBertDestroy(void *program) {
     release(p->result_slot[i], true);
   }
   for (Tensor &w : p->weights) release(w, true);
+  for (Coded &w : p->coded) release(w);
+  release(p->coded_hidden);
+  release(p->coded_ffn);
+  release(p->rotated, false);
+  release(p->frequencies, false);
   release(p->x, true);
   release(p->type_rows, true);
   release(p->qkv, true);
@@ -346,6 +436,7 @@ int homBertSetWeight(void *program, int32_t index, int64_t rank, void *descripto
       rank != 3)
     return HOM_ERR_INVALID;
   release(p->weights[index], true);
+  p->coded_stale = true;
   // Copy the descriptor record so the caller's may go away; the buffer stays the caller's.
   const size_t bytes = sizeof(int64_t) * (3 + 2 * rank);
   void *copy = std::malloc(bytes);
@@ -374,12 +465,81 @@ int homBertSetWeight(void *program, int32_t index, int64_t rank, void *descripto
 int homBertLoadConstants(void *program, int32_t first_idx) {
   auto *p = static_cast<Program *>(program);
   if (!p) return HOM_ERR_INVALID;
+  p->coded_stale = true;
   for (size_t i = 0; i < p->weights.size(); ++i) {
     release(p->weights[i], true);
     HomUnrankedMemRef m = allocConstantNVGPUF16(first_idx + static_cast<int32_t>(i));
     if (status() != 0 || !m.descriptor) return status() ? status() : HOM_ERR_IO;
     p->weights[i] = from_alloc(m);
   }
+  return 0;
+}
+
+int homBertQuantizeWeights(void *program) {
+  auto *p = static_cast<Program *>(program);
+  if (!p || p->cfg.fused_layernorm != 0) return HOM_ERR_INVALID;
+  for (const Tensor &w : p->weights)
+    if (!w.desc) return HOM_ERR_INVALID;
+  const HomBertConfig &c = p->cfg;
+  const int64_t rows = static_cast<int64_t>(c.batch) * c.seq;
+  forget_graphs(*p);
+  std::vector<Coded> coded(static_cast<size_t>(4) * c.layers);
+  Coded hidden, ffn;
+  bool ok = make_coded(rows, c.hidden, &hidden) && make_coded(rows, c.ffn, &ffn);
+  for (size_t i = 0; ok && i < coded.size(); ++i) {
+    Tensor &w = p->weights[3 + i];
+    const int64_t *words = static_cast<const int64_t *>(w.desc);  // [1, K, N], or [1, N, K]
+    const int64_t n = words[c.weights_nk ? 4 : 5], k = words[c.weights_nk ? 5 : 4];
+    ok = make_coded(n, k, &coded[i]);
+    if (!ok) break;
+    homQuantizeMxF4F16(w.rank, w.desc, c.weights_nk == 0, coded[i].codes.rank, coded[i].codes.desc, coded[i].scales.rank,
+                       coded[i].scales.desc);
+    declare(coded[i].codes);
+    declare(coded[i].scales);
+  }
+  // (also waits for the forwards that still read what was quantised before)
+  const int rc = homSynchronize();
+  for (Coded &w : p->coded) release(w);
+  release(p->coded_hidden);
+  release(p->coded_ffn);
+  p->coded.clear();
+  if (!ok || rc != 0) {
+    for (Coded &w : coded) release(w);
+    release(hidden);
+    release(ffn);
+    return rc != 0 ? rc : HOM_ERR_CUDA;
+  }
+  p->coded = coded;
+  p->coded_stale = false;
+  p->coded_hidden = hidden;
+  p->coded_ffn = ffn;
+  return 0;
+}
+
+int homBertSetRotary(void *program, double base, int32_t scaling, double factor, double originalLength, double betaFast,
+                     double betaSlow, float magnitude) {
+  auto *p = static_cast<Program *>(program);
+  const int64_t d = p ? p->cfg.hidden / p->cfg.heads : 0;
+  if (!p || d % 2 != 0 || !std::isfinite(magnitude)) return HOM_ERR_INVALID;
+  const HomBertConfig &c = p->cfg;
+  forget_graphs(*p);
+  Tensor f = make_bytes({d / 2 * 8});
+  if (!f.data()) return status() ? status() : HOM_ERR_CUDA;
+  static_cast<int64_t *>(f.desc)[3] = d / 2;  // the same memory as fp64 [d / 2]
+  homRotaryFrequencies(f.rank, f.desc, base, scaling, factor, originalLength, betaFast, betaSlow);
+  const int rc = homSynchronize();
+  release(p->frequencies, false);
+  release(p->rotated, false);
+  if (rc != 0) {
+    release(f, false);
+    return rc;
+  }
+  p->frequencies = f;
+  p->rotary_magnitude = magnitude;
+  p->rotated = make_view(p->qkv.data(), {c.batch, c.seq, 2 * c.heads, d});
+  int64_t *w = static_cast<int64_t *>(p->rotated.desc);
+  w[7] = static_cast<int64_t>(c.seq) * 3 * c.hidden;  // strides of the packed buffer
+  w[8] = static_cast<int64_t>(3) * c.hidden;
   return 0;
 }
 
@@ -458,8 +618,7 @@ int homBertForwardHostAsync(void *program, const int64_t *ids_host, const int64_
                                            static_cast<long long>(out_bytes / 16));
     return cudaGetLastError() == cudaSuccess ? 0 : HOM_ERR_CUDA;
   };
-  for (const Tensor &w : p->weights)
-    if (!w.desc) return HOM_ERR_INVALID;
+  if (!ready(*p)) return HOM_ERR_INVALID;
   if (!pinned_inputs) {
     // Pageable host memory cannot be read by a kernel, and copies from it cannot be captured:
     // copy eagerly, then the (possibly graph-replayed) call sequence and the slot copy.
@@ -541,7 +700,8 @@ int32_t homBertLaunchesPerForward(void *program) {
   if (!p) return 0;
   const int per_layer = p->cfg.fused_layernorm ? 5 : 7;
   const int tail = p->cfg.fused_layernorm == 2 && p->cfg.layers > 0 ? 1 : 0;  // the final LayerNorm
-  return (p->cfg.fused_embedding ? 2 : 6) + per_layer * p->cfg.layers + tail;
+  const int more = (p->coded.empty() ? 0 : 4) + (p->frequencies.desc ? 1 : 0);  // quantised activations, rotation
+  return (p->cfg.fused_embedding ? 2 : 6) + (per_layer + more) * p->cfg.layers + tail;
 }
 
 }  // extern "C"

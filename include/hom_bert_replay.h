@@ -67,6 +67,19 @@ HOM_EXPORT int homBertSetWeight(void *program, int32_t index, int64_t rank, void
  * init function does; the program owns (and frees) those buffers. */
 HOM_EXPORT int homBertLoadConstants(void *program, int32_t first_idx);
 
+/* From now on the four projections of every layer are computed in microscaled 4-bit floating point:
+ * homQuantizeMxF4F16 of the activations, then homGemmMxF4F16 with the weights that this call
+ * quantises from those bound now (which stay bound).  After other weights were bound, forwards are
+ * refused until this is called again; call it too after rewriting a weight in place.  Needs
+ * fused_layernorm == 0.  Waits for the stream. */
+HOM_EXPORT int homBertQuantizeWeights(void *program);
+
+/* From now on homRotaryF16 turns the queries and keys of every layer by their positions, over whole
+ * heads, with the frequencies that homRotaryFrequencies makes of these arguments.  The position
+ * table still takes part: a model without one binds zeros.  Waits for the stream. */
+HOM_EXPORT int homBertSetRotary(void *program, double base, int32_t scaling, double factor, double originalLength,
+                                double betaFast, double betaSlow, float magnitude);
+
 /* Enqueues one forward on the library's current stream.  ids / mask / token types are
  * int64 [batch, seq] device memrefs; *result receives the descriptor of the program-owned
  * final hidden states, fp16 [batch, seq, hidden].  use_graph != 0 captures the call sequence
