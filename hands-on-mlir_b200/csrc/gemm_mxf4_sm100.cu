@@ -207,6 +207,21 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int t = threadIdx.x - 64;
     constexpr int kPieces = BN / 8;  // 8-column pieces of an output row
     constexpr int kTasks = ALIGNED ? BM * kPieces / kExchangeThreads : 1;
+    // not aligned: one column per thread and every fourth row, a batch of them at a time; C's values of
+    // the first batch are asked for now, like the pieces above
+    constexpr int kRowStep = kExchangeThreads / BN, kRows = 16;
+    const int column = t % BN, col = n0 + column;
+    unsigned short c_bits[ALIGNED ? 1 : kRows];
+    auto load_c = [&](int base) {
+      const unsigned short *c = reinterpret_cast<const unsigned short *>(p.C) + col +
+                                (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + base) * p.N : 0);
+      const long long step = p.c_mode == 1 ? static_cast<long long>(kRowStep) * p.N : 0;
+#pragma unroll
+      for (int i = 0; i < (ALIGNED ? 1 : kRows); ++i) {
+        c_bits[i] = p.c_mode != 0 && base + i * kRowStep < my_rows && col < p.N ? *c : 0;
+        c += step;
+      }
+    };
 
     pdl_wait();  // C may be produced, and D still read, by the previous kernel
     uint4 cval[kTasks];
@@ -219,6 +234,8 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           cval[i] = *reinterpret_cast<const uint4 *>(
               p.C + (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + row) * p.N : 0) + col);
       }
+    } else {
+      load_c(t / BN);
     }
     bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, kDevWaitTimeoutEpilogue);
     ok = __all_sync(0xffffffffu, ok);
@@ -291,37 +308,32 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
         }
       } else {
-        // one column per thread, eight rows of C in flight
-        const int column = t % BN, col = n0 + column;
         const uint32_t at = smem_base + kRecv + (column & 3) * 4;
-        constexpr int kRowStep = kExchangeThreads / BN;
-        if (col < p.N) {
-          for (int base = t / BN; base < my_rows; base += 8 * kRowStep) {
-            float c[8];
+        for (int base = t / BN; base < my_rows; base += kRows * kRowStep) {
+          if (base >= kRowStep) load_c(base);
+          float v[kRows];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int local = base + i * kRowStep;
-              c[i] = p.c_mode != 0 && local < my_rows
-                         ? __half2float(p.C[(p.c_mode == 1 ? static_cast<long long>(m0 + row_first + local) * p.N : 0) + col])
-                         : 0.f;
+          for (int i = 0; i < kRows; ++i) v[i] = 0.f;
+          for (int q = 0; q < parts; ++q) {
+            float f[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+              const int local = min(base + i * kRowStep, my_rows - 1);
+              asm volatile("ld.shared.f32 %0, [%1];"
+                           : "=f"(f[i])
+                           : "r"(at + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
+                                 (static_cast<uint32_t>(column >> 2) ^ (local & 7)) * 16));
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int local = base + i * kRowStep;
-              if (local >= my_rows) break;
-              float v = 0.f;
-              for (int q = 0; q < parts; ++q) {
-                float f;
-                asm volatile("ld.shared.f32 %0, [%1];"
-                             : "=f"(f)
-                             : "r"(at + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
-                                   (static_cast<uint32_t>(column >> 2) ^ (local & 7)) * 16)
-                             : "memory");
-                v += f;
-              }
-              p.D[static_cast<long long>(m0 + row_first + local) * p.N + col] =
-                  __float2half_rn(epilogue2(p, make_float2(v, 0.f), make_float2(c[i], 0.f)).x);
-            }
+            for (int i = 0; i < kRows; ++i) v[i] += f[i];
+          }
+          __half *d = p.D + static_cast<long long>(m0 + row_first + base) * p.N + col;
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const float2 r = epilogue2(p, make_float2(v[i], 0.f),
+                                       make_float2(__half2float(__ushort_as_half(c_bits[i])), 0.f));
+            if (base + i * kRowStep < my_rows && col < p.N) *d = __float2half_rn(r.x);
+            d += static_cast<long long>(kRowStep) * p.N;
           }
         }
       }
