@@ -133,41 +133,52 @@ __device__ __forceinline__ void finish_half(const Params &p, const uint32_t (&ac
   const float2 alpha2 = make_float2(p.alpha, p.alpha), beta2 = make_float2(p.beta, p.beta);
   const bool full = general(FORM) ? p.c_mode == 1 : (FORM & kFull) != 0;
   const bool row = general(FORM) ? p.c_mode == 2 : (FORM & kRow) != 0;
+  constexpr int kChunks = 2;  // 16-byte pieces of the staging row at a time
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const uint32_t addr = my_row + ((static_cast<uint32_t>(half * 4 + g) ^ (lane & 7u)) << 4);
-    float2 c[4];
-    if (full || (row && general(FORM))) {
-      uint32_t h[4];
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-                   : "r"(full ? addr : bias + (half * 4 + g) * 16)
-                   : "memory");
+  for (int g = 0; g < 4; g += kChunks) {
+    float2 v[4 * kChunks];
+    uint32_t addr[kChunks];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-    } else if (row) {
-#pragma unroll
-      for (int j = 0; j < 4; j += 2)
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(c[j].x), "=f"(c[j].y), "=f"(c[j + 1].x), "=f"(c[j + 1].y)
-                     : "r"(bias + (half * 32 + g * 8 + j * 2) * 4)
+    for (int h = 0; h < kChunks; ++h) {
+      addr[h] = my_row + ((static_cast<uint32_t>(half * 4 + g + h) ^ (lane & 7u)) << 4);
+      float2 c[4];
+      if (full || (row && general(FORM))) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(full ? addr[h] : bias + (half * 4 + g + h) * 16)
                      : "memory");
-    }
-    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * 8 + 2 * j;
-      float2 v = make_float2(__uint_as_float(acc[i]), __uint_as_float(acc[i + 1]));
-      if (general(FORM)) v = __fmul2_rn(alpha2, v);
-      if (full || row) {
-        v = general(FORM) ? __ffma2_rn(beta2, c[j], v) : __fadd2_rn(c[j], v);
+        for (int j = 0; j < 4; ++j) c[j] = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+      } else if (row) {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(c[j].x), "=f"(c[j].y), "=f"(c[j + 1].x), "=f"(c[j + 1].y)
+                       : "r"(bias + (half * 32 + (g + h) * 8 + j * 2) * 4)
+                       : "memory");
       }
-      if (general(FORM) ? p.act == 1 : (FORM & kGelu) != 0) v = gelu2(v);
-      const __half2 h = __floats2half2_rn(v.x, v.y);
-      w[j] = *reinterpret_cast<const uint32_t *>(&h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = (g + h) * 8 + 2 * j;
+        float2 x = make_float2(__uint_as_float(acc[i]), __uint_as_float(acc[i + 1]));
+        if (general(FORM)) x = __fmul2_rn(alpha2, x);
+        if (full || row) x = general(FORM) ? __ffma2_rn(beta2, c[j], x) : __fadd2_rn(c[j], x);
+        v[4 * h + j] = x;
+      }
     }
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                 : "memory");
+    if (general(FORM) ? p.act == 1 : (FORM & kGelu) != 0) gelu2(v);
+#pragma unroll
+    for (int h = 0; h < kChunks; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2 r = __floats2half2_rn(v[4 * h + j].x, v[4 * h + j].y);
+        w[j] = *reinterpret_cast<const uint32_t *>(&r);
+      }
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr[h]), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
   }
 }
 

@@ -130,7 +130,11 @@ __global__ void __launch_bounds__(32 * kWarps) gemm_mxf4_rows_kernel(const Param
     if (lane == m) {
       float v = p.alpha * sum[m];
       if (p.c != nullptr) v = fmaf(p.beta, __half2float(p.c[m * p.c_pitch + n]), v);
-      if (p.act == 1) v = gelu2(make_float2(v, 0.f)).x;
+      if (p.act == 1) {
+        float2 x[1] = {make_float2(v, 0.f)};
+        gelu2(x);
+        v = x[0].x;
+      }
       p.d[static_cast<long long>(m) * p.n + n] = __float2half_rn(v);
     }
   }

@@ -71,7 +71,12 @@ __device__ __forceinline__ uint32_t cluster_nctas() {
 __device__ __forceinline__ float2 epilogue2(const Params &p, float2 v, float2 c) {
   v = __fmul2_rn(make_float2(p.alpha, p.alpha), v);
   if (p.c_mode != 0) v = __ffma2_rn(make_float2(p.beta, p.beta), c, v);
-  return p.act == 1 ? gelu2(v) : v;
+  if (p.act == 1) {
+    float2 x[1] = {v};
+    gelu2(x);
+    return x[0];
+  }
+  return v;
 }
 
 // ALIGNED: N % 8 == 0, rows of C and D travel in 16-byte pieces; otherwise element by element,
