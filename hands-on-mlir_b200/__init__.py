@@ -9,6 +9,8 @@ from the compiled model.  There is no CPU fallback: a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from ctypes import c_bool, c_char_p, c_double, c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
@@ -19,6 +21,7 @@ PKG_DIR = Path(__file__).resolve().parent
 _LIB_DIR = Path(os.environ["HOM_LIB_DIR"]).resolve() if os.environ.get("HOM_LIB_DIR") else PKG_DIR / "lib"
 RUNNER_LIB = _LIB_DIR / "libhands_on_mlir_nvgpu_runner_utils.so"
 REPLAY_LIB = _LIB_DIR / "libhom_bert_replay.so"
+CALLS_MODULE = _LIB_DIR / "hom_calls.so"
 
 
 class HomError(RuntimeError):
@@ -70,6 +73,7 @@ class MemRef:
         # built once: the cast costs more than the rest of a call's argument conversion (it also
         # keeps the words alive for a caller that only holds `args`)
         self.args = c_int64(rank), ctypes.cast(self._words, c_void_p)
+        self.address = ctypes.addressof(self._words)
 
     @classmethod
     def of(cls, tensor) -> "MemRef":
@@ -186,10 +190,26 @@ def mxf4_shapes(rows: int, cols: int) -> tuple[tuple[int, int], tuple[int, int, 
     return (rows, 16 * blocks), (-(-rows // 128), -(-blocks // 4), 512)
 
 
+def _direct_calls(path: Path):
+    """The optional module of direct calls beside the library at `path`, or None.  It calls the
+    library that the process has loaded under that file name."""
+    module = path.parent / CALLS_MODULE.name
+    if not module.exists() or path.resolve() != RUNNER_LIB.resolve():
+        return None
+    try:
+        loader = importlib.machinery.ExtensionFileLoader("hom_calls", str(module))
+        calls = importlib.util.module_from_spec(importlib.util.spec_from_loader("hom_calls", loader))
+        loader.exec_module(calls)
+    except ImportError:
+        return None
+    calls.bind(MemRef, MemRef.of)
+    return calls
+
+
 class RunnerUtils:
     """ctypes view of libhands_on_mlir_nvgpu_runner_utils.so with error checking."""
 
-    def __init__(self, path: Path | str = RUNNER_LIB):
+    def __init__(self, path: Path | str = RUNNER_LIB, direct: bool = True):
         path = Path(path)
         if not path.exists():
             raise FileNotFoundError(
@@ -201,6 +221,7 @@ class RunnerUtils:
             fn = getattr(self.lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
+        self._calls = _direct_calls(path) if direct else None
 
     # ------------------------------------------------------------ error channel
     def check(self):
@@ -301,32 +322,60 @@ class RunnerUtils:
         self.check()
 
     def homQuantizeMxF4F16(self, X, Q, S, transposed=False):
+        if self._calls:
+            if self._calls.homQuantizeMxF4F16(X, Q, S, transposed):
+                self.check()
+            return
         self.lib.homQuantizeMxF4F16(*_as_args(X), transposed, *_as_args(Q), *_as_args(S))
         self.check()
 
     def homQuantizeMxF4F32(self, X, Q, S, transposed=False):
+        if self._calls:
+            if self._calls.homQuantizeMxF4F32(X, Q, S, transposed):
+                self.check()
+            return
         self.lib.homQuantizeMxF4F32(*_as_args(X), transposed, *_as_args(Q), *_as_args(S))
         self.check()
 
     def homDequantizeMxF4F16(self, Q, S, Out):
+        if self._calls:
+            if self._calls.homDequantizeMxF4F16(Q, S, Out):
+                self.check()
+            return
         self.lib.homDequantizeMxF4F16(*_as_args(Q), *_as_args(S), *_as_args(Out))
         self.check()
 
     def homDequantizeMxF4F32(self, Q, S, Out):
+        if self._calls:
+            if self._calls.homDequantizeMxF4F32(Q, S, Out):
+                self.check()
+            return
         self.lib.homDequantizeMxF4F32(*_as_args(Q), *_as_args(S), *_as_args(Out))
         self.check()
 
     def homGemmMxF4F16(self, A, SA, B, SB, C, D, activation=0, alpha=1.0, beta=0.0):
+        if self._calls:
+            if self._calls.homGemmMxF4F16(A, SA, B, SB, C, D, activation, alpha, beta):
+                self.check()
+            return
         self.lib.homGemmMxF4F16(*_as_args(A), *_as_args(SA), *_as_args(B), *_as_args(SB), *_as_args(C),
                                 *_as_args(D), activation, alpha, beta)
         self.check()
 
     def homRotaryF16(self, X, positions, frequencies, Out, interleaved=False, backward=False, magnitude=1.0):
+        if self._calls:
+            if self._calls.homRotaryF16(X, positions, frequencies, Out, interleaved, backward, magnitude):
+                self.check()
+            return
         self.lib.homRotaryF16(*_as_args(X), *_as_args(positions), *_as_args(frequencies), *_as_args(Out),
                               interleaved, backward, magnitude)
         self.check()
 
     def homRotaryF32(self, X, positions, frequencies, Out, interleaved=False, backward=False, magnitude=1.0):
+        if self._calls:
+            if self._calls.homRotaryF32(X, positions, frequencies, Out, interleaved, backward, magnitude):
+                self.check()
+            return
         self.lib.homRotaryF32(*_as_args(X), *_as_args(positions), *_as_args(frequencies), *_as_args(Out),
                               interleaved, backward, magnitude)
         self.check()

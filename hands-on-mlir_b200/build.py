@@ -7,6 +7,8 @@
                                                library the reference builds in
                                                lib/CMakeLists.txt:40-55)
   lib/libhom_bert_replay.so                    the BERT call-sequence replay program
+  lib/hom_calls.so                             direct calls for the Python binding (where the
+                                               interpreter's headers are; optional)
 
 nvcc cross-compiles without a GPU, so this also runs on a CPU-only machine.
 
@@ -21,6 +23,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -32,6 +35,7 @@ OBJ_DIR = PKG_DIR / "build"
 INCLUDE = REPO_DIR / "include"
 
 RUNNER_LIB = LIB_DIR / "libhands_on_mlir_nvgpu_runner_utils.so"
+CALLS_MODULE = "hom_calls.so"
 REPLAY_LIB = LIB_DIR / "libhom_bert_replay.so"
 
 RUNNER_SOURCES = [
@@ -95,6 +99,25 @@ def _link(objs: list[Path], out: Path, extra: list[str], verbose: bool) -> None:
         raise RuntimeError(f"link failed for {out.name}:\n{proc.stdout}\n{proc.stderr}")
 
 
+def _build_calls(lib_dir: Path, runner_lib: Path, force: bool, verbose: bool) -> None:
+    """The optional module that spares the Python binding ctypes' argument conversion."""
+    src, out = CSRC / "py_calls.c", lib_dir / CALLS_MODULE
+    headers = Path(sysconfig.get_paths()["include"])
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if not (headers / "Python.h").exists() or not cc:
+        print("hom_calls: no Python.h or C compiler, the binding uses ctypes")
+        return
+    if not force and out.exists() and out.stat().st_mtime > max(src.stat().st_mtime, _newest_header_mtime()):
+        return
+    cmd = [cc, "-O2", "-shared", "-fPIC", "-fvisibility=hidden", f"-I{headers}", f"-I{INCLUDE}", str(src), "-o", str(out),
+           f"-L{lib_dir}", "-lhands_on_mlir_nvgpu_runner_utils", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"building {out.name} failed:\n{proc.stdout}\n{proc.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False, diagnostics: bool = False) -> dict[str, Path]:
     """Compile what is out of date and return the paths of the two libraries."""
     lib_dir = LIB_DIR / "diagnostics" if diagnostics else LIB_DIR
@@ -124,6 +147,7 @@ def build(force: bool = False, verbose: bool = False, diagnostics: bool = False)
     runner_objs = [objs[n] for n in RUNNER_SOURCES if n in objs]
     if force or jobs or not runner_lib.exists():
         _link(runner_objs, runner_lib, [], verbose)
+    _build_calls(lib_dir, runner_lib, force, verbose)
     replay_objs = [objs[n] for n in REPLAY_SOURCES if n in objs]
     if replay_objs and (force or jobs or not replay_lib.exists()):
         _link(replay_objs, replay_lib,

@@ -150,3 +150,34 @@ def test_calls_without_elements_have_no_effect(pkg, hom, nothing_launched):
         x = torch.empty(shape, dtype=torch.float32)
         hom.homRotaryF32(x, None, f, x)
         hom.homRotaryF32(x, torch.empty(shape[:2], dtype=torch.int64), f, x)
+
+
+def test_direct_calls_and_ctypes_agree(pkg, hom, nothing_launched):
+    """The two ways the binding has of calling: the same refusals, argument errors as exceptions, tensors or descriptors."""
+    import torch
+
+    through = [pkg.RunnerUtils(direct=False)]
+    assert through[0]._calls is None
+    if pkg.CALLS_MODULE.exists():
+        assert hom._calls is not None
+        through.append(hom)
+    q, s = _coded(pkg, 5, 40)
+    x, rot = torch.zeros((5, 41), dtype=torch.float16), _host(pkg, (2, 3, 4, 8), 2)
+    a, b = _coded(pkg, 6, 64), _coded(pkg, 16, 64)
+    empty = [torch.empty(shape, dtype=torch.uint8) for shape in pkg.mxf4_shapes(0, 64)]
+    for h in through:
+        _refused(pkg, 1, "need codes", h.homQuantizeMxF4F16, torch.zeros((5, 70), dtype=torch.float16), q, s)
+        _refused(pkg, 1, "need codes", h.homQuantizeMxF4F32, x, q, s, transposed=True)
+        _refused(pkg, 1, "do not hold", h.homDequantizeMxF4F16, q, s, torch.zeros((5, 70), dtype=torch.float16))
+        _refused(pkg, 1, "do not hold", h.homDequantizeMxF4F32, q, s, _host(pkg, (6, 40), 4))
+        _refused(pkg, 2, "activation 5", h.homGemmMxF4F16, *a, *b, None, _host(pkg, (6, 16), 2), activation=5)
+        _refused(pkg, 1, "needs a contiguous C", h.homGemmMxF4F16, *a, *b, None, _host(pkg, (6, 16), 2), beta=1)
+        _refused(pkg, 1, "Frequencies", h.homRotaryF16, rot, None, None, rot)
+        _refused(pkg, 1, "magnitude", h.homRotaryF32, rot, None, _host(pkg, (4,), 8), rot, magnitude=float("inf"))
+        h.homQuantizeMxF4F16(torch.empty((0, 64), dtype=torch.float16), *empty)
+        with pytest.raises(Exception) as e:
+            h.homQuantizeMxF4F16("no tensor", q, s)
+        assert not isinstance(e.value, pkg.HomError)
+        with pytest.raises(Exception) as e:
+            h.homGemmMxF4F16(*a, *b, None, _host(pkg, (6, 16), 2), alpha="one")
+        assert not isinstance(e.value, pkg.HomError)
