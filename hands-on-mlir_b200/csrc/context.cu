@@ -60,6 +60,7 @@ DeviceState &device_state() {
   if (dev < 0 || dev >= kMaxDevices) dev = 0;
   DeviceState &st = g_devices[dev];
   std::call_once(st.once, [&st, dev]() {
+    CaptureSafeCalls safe;  // the first call on a device may be a captured one
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) == cudaSuccess) st.sm_count = prop.multiProcessorCount;
     void *host = nullptr;

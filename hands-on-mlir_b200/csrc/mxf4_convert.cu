@@ -158,8 +158,9 @@ struct Eight<float> {
 // 128-row group: four independent loads in flight, and the scales of the four rows are the 16
 // consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED: rows
 // start on 16 bytes (cols % 8 == 0); otherwise the warp reads element by element, coalesced, and
-// sorts the values through shared memory.  (A persistent form that requests the next unit's values
-// early was slower: its registers cost more loads in flight than it gains.)
+// sorts the values through shared memory.  (Slower: a persistent form that requests the next unit's
+// values early, whose registers cost more loads in flight than it gains; fp32 values of ragged rows
+// by 4-byte asynchronous copies, 20011 x 777 of them in 19.6 us instead of 16.6.)
 //
 // What the rows kernel needs is many loads in flight, so its registers are held down: 65536 x 4096
 // fp16 values 119 us with room for five CTAs on an SM, 112 for eight (6.0 TB/s); 20011 x 776 fp32
@@ -234,7 +235,8 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
 // x stored [cols, rows]: a thread owns one block of COLUMNS rows of the result, that is 32 values of
 // as many columns of x, all of them in flight; neighbouring threads read neighbouring elements.  A
 // CTA makes one scale tile, whose bytes it gathers in shared memory.  Two columns for fp16 (rows even,
-// x on 4 bytes): with 2-byte loads a 4096 x 4096 weight took 27.7 us.
+// x on 4 bytes): a [4096, 4096] weight takes 14.1 us (3.0 TB/s: pieces of 256 bytes out of rows of
+// 8 KB), with 2-byte loads 27.7.
 template <typename T, int COLUMNS>
 __global__ void __launch_bounds__(kTileRows * kTileBlocks / COLUMNS)
 quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks) {
@@ -258,12 +260,22 @@ quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long r
       for (int c = 0; c < COLUMNS; ++c) v[j].v[c] = T(0.f);
     }
   }
+  uint32_t largest[COLUMNS];
+  if constexpr (COLUMNS == 2) {
+    // both columns' maxima at once
+    __half2 m = __float2half2_rn(0.f);
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2 *>(&v[j])));
+    largest[0] = magnitude_bits(__low2float(m));
+    largest[1] = magnitude_bits(__high2float(m));
+  } else {
+    largest[0] = 0;
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) largest[0] = max(largest[0], magnitude_bits(to_float(v[j].v[0])));
+  }
 #pragma unroll
   for (int c = 0; c < COLUMNS; ++c) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int j = 0; j < kBlock; ++j) bits = max(bits, magnitude_bits(to_float(v[j].v[c])));
-    const uint32_t byte = scale_byte(bits);
+    const uint32_t byte = scale_byte(largest[c]);
     const float inv = reciprocal_scale(byte);
     uint32_t packed[4];
 #pragma unroll
@@ -286,12 +298,15 @@ quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long r
         reinterpret_cast<const uint4 *>(tile_bytes)[t];
 }
 
-// The way back, with the same division of work.
+// The way back, with the same division of work.  Where a lane's eight values are more than 16 bytes
+// (fp32), or rows start anywhere, they go through shared memory, so that a store of the warp covers
+// consecutive bytes (20011 x 776 fp32 values: two half-filled stores a lane 16.4 us).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kWarps)
 dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *out,
                   long long rows, int cols, int blocks, int segments, long long units) {
-  __shared__ float sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 4 : kSegment];
+  constexpr bool kDirect = ALIGNED && sizeof(T) == 2;
+  __shared__ __align__(16) float sorted[kDirect ? 1 : kWarps][kDirect ? 4 : kSegment];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -328,16 +343,26 @@ dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *out,
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= scale;
     T *dst = out + row * cols;
-    if (ALIGNED) {
+    if constexpr (kDirect) {
       if (col < cols) store8(dst + col, v);
     } else {
       __syncwarp();
       store8(&sorted[warp][lane * kLaneValues], v);
       __syncwarp();
+      if constexpr (ALIGNED) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = segment * kSegment + j * 32 + lane;
-        if (c < cols) store1(dst + c, sorted[warp][j * 32 + lane]);
+        for (int h = 0; h < 2; ++h) {
+          const int c = segment * kSegment + h * (kSegment / 2) + lane * 4;
+          if (c < cols)
+            *reinterpret_cast<float4 *>(dst + c) =
+                *reinterpret_cast<const float4 *>(&sorted[warp][h * (kSegment / 2) + lane * 4]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = segment * kSegment + j * 32 + lane;
+          if (c < cols) store1(dst + c, sorted[warp][j * 32 + lane]);
+        }
       }
     }
   }

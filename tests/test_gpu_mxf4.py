@@ -133,7 +133,8 @@ def _product(hom, cuda, a, sa, b, sb, c, d, act=0, alpha=1.0, beta=0.0):
 # is no multiple of 8 in each
 PRODUCTS = [(1, 8, 32), (1, 4096, 1024), (2, 1, 32), (2, 333, 5000), (7, 33, 96), (16, 768, 4096), (33, 77, 2100),
             (127, 129, 256), (128, 128, 288), (129, 200, 544), (385, 1001, 808), (300, 1000, 800), (640, 512, 1056),
-            (1100, 2304, 768), (2500, 1024, 520), (1001, 2001, 1060), (3900, 2400, 300), (4001, 2391, 600)]
+            (1100, 2304, 768), (2500, 1024, 520), (1001, 2001, 1060), (3900, 2400, 300), (4001, 2391, 600),
+            (5, 72, 40000), (900, 1288, 2500)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -305,3 +306,41 @@ def test_streams_graphs_and_declared_weights(hom, pkg, cuda):
         hom.use_torch_stream()
         hom.forget_weights(bq)
         hom.forget_weights(bs)
+
+
+def test_two_threads_on_two_streams(hom, pkg, cuda):
+    """Calls of two host threads overlap on the device and in the library."""
+    import threading
+
+    import torch
+
+    rng = np.random.default_rng(21)
+    jobs = []
+    for m, n, k in ((1, 512, 768), (96, 328, 1280), (3000, 2304, 768), (500, 2403, 640)):
+        a, sa, b, sb = (to_dev(t, cuda) for t in _operands(rng, m, n, k, 2))
+        want = torch.empty((m, n), dtype=torch.float16, device=cuda)
+        hom.homGemmMxF4F16(a, sa, b, sb, None, want, 1, 0.01)
+        jobs.append(((a, sa, b, sb), want))
+    hom.synchronize()
+    bad = []
+
+    def work(order):
+        stream = torch.cuda.Stream()
+        hom.set_stream(stream.cuda_stream)
+        outs = []
+        for _ in range(10):
+            for i in order:
+                operands, want = jobs[i]
+                with torch.cuda.stream(stream):
+                    d = torch.empty_like(want)
+                hom.homGemmMxF4F16(*operands, None, d, 1, 0.01)
+                outs.append((i, d))
+        hom.synchronize()
+        bad.extend(i for i, d in outs if not torch.equal(d, jobs[i][1]))
+
+    threads = [threading.Thread(target=work, args=(order,)) for order in ((0, 1, 2, 3), (3, 2, 1, 0))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
