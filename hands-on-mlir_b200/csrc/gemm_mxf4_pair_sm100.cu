@@ -224,16 +224,15 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     prefetch_tensormap(&tmSA);
     prefetch_tensormap(&tmD);
   }
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < 4 * kStages; ++s) mbar_init(bar_base + 8 * s, 1);
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(acc_full_bar(a), 1);
-      mbar_init(acc_empty_bar(a), 2 * kDrainWarps);
+  if (warp == 0) {
+    for (int i = lane; i < kBarriers; i += 32) {
+      const uint32_t bar = bar_base + 8 * i;
+      const bool acc_empty = bar == acc_empty_bar(0) || bar == acc_empty_bar(1);
+      mbar_init(bar, bar == shared_bar ? 2 * 4 * kSharingGroups : acc_empty ? 2 * kDrainWarps : 1);
     }
-    mbar_init(shared_bar, 2 * 4 * kSharingGroups);
-    for (int w = 0; w < kDrainWarps; ++w) mbar_init(c_bar(w), 1);
-    *abort_flag = 0;
+    if (lane == 0) *abort_flag = 0;
     fence_mbar_init();
+    __syncwarp();
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(const_cast<uint32_t *>(tmem_slot)), kTmemCols);
