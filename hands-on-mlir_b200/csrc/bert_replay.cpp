@@ -499,16 +499,15 @@ int homBertQuantizeWeights(void *program) {
   }
   // (also waits for the forwards that still read what was quantised before)
   const int rc = homSynchronize();
-  for (Coded &w : p->coded) release(w);
-  release(p->coded_hidden);
-  release(p->coded_ffn);
-  p->coded.clear();
-  if (!ok || rc != 0) {
+  if (!ok || rc != 0) {  // nothing changes
     for (Coded &w : coded) release(w);
     release(hidden);
     release(ffn);
     return rc != 0 ? rc : HOM_ERR_CUDA;
   }
+  for (Coded &w : p->coded) release(w);
+  release(p->coded_hidden);
+  release(p->coded_ffn);
   p->coded = coded;
   p->coded_stale = false;
   p->coded_hidden = hidden;
@@ -528,12 +527,12 @@ int homBertSetRotary(void *program, double base, int32_t scaling, double factor,
   static_cast<int64_t *>(f.desc)[3] = d / 2;  // the same memory as fp64 [d / 2]
   homRotaryFrequencies(f.rank, f.desc, base, scaling, factor, originalLength, betaFast, betaSlow);
   const int rc = homSynchronize();
-  release(p->frequencies, false);
-  release(p->rotated, false);
-  if (rc != 0) {
+  if (rc != 0) {  // nothing changes
     release(f, false);
     return rc;
   }
+  release(p->frequencies, false);
+  release(p->rotated, false);
   p->frequencies = f;
   p->rotary_magnitude = magnitude;
   p->rotated = make_view(p->qkv.data(), {c.batch, c.seq, 2 * c.heads, d});

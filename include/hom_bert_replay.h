@@ -71,7 +71,8 @@ HOM_EXPORT int homBertLoadConstants(void *program, int32_t first_idx);
  * homQuantizeMxF4F16 of the activations, then homGemmMxF4F16 with the weights that this call
  * quantises from those bound now (which stay bound).  After other weights were bound, forwards are
  * refused until this is called again; call it too after rewriting a weight in place.  Needs
- * fused_layernorm == 0.  Waits for the stream. */
+ * fused_layernorm == 0.  Waits for the stream.  A refused call changes nothing, nor does one of
+ * homBertSetRotary. */
 HOM_EXPORT int homBertQuantizeWeights(void *program);
 
 /* From now on homRotaryF16 turns the queries and keys of every layer by their positions, over whole

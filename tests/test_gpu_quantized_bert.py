@@ -207,6 +207,26 @@ def test_program_with_quantized_projections(hom, pkg, cuda, nk):
     prog.close()
 
 
+def test_a_refused_option_changes_nothing(hom, pkg, cuda):
+    from hands_on_mlir_b200.bert_program import BertProgram
+
+    cfg, w, rng = _model(4, 16, layers=1)
+    args = [to_dev(v, cuda) for v in _inputs(cfg, rng, [16, 5], 16)]
+    prog = BertProgram(cfg, 2, 16)
+    prog.set_weights({k: to_dev(v, cuda) for k, v in w.items()})
+    plain = prog.result_to_torch(prog.forward(*args)).cpu().numpy()
+    prog.set_rotary(base=100.0, magnitude=1.2)
+    prog.quantize_weights()
+    want = prog.result_to_torch(prog.forward(*args, use_graph=True)).cpu().numpy()
+    assert not np.array_equal(plain, want)
+    for bad in (dict(base=-1.0), dict(scaling="linear", factor=0.0), dict(magnitude=float("inf"))):
+        with pytest.raises(pkg.HomError):
+            prog.set_rotary(**bad)
+        for graph in (True, True):
+            assert_bits_equal(prog.result_to_torch(prog.forward(*args, use_graph=graph)).cpu().numpy(), want, str(bad))
+    prog.close()
+
+
 def test_program_refusals_and_new_weights(hom, pkg, cuda):
     from hands_on_mlir_b200.bert_program import BertProgram
 
