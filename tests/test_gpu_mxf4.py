@@ -250,6 +250,44 @@ def test_extreme_scales(hom, cuda):
         assert np.array_equal(d.cpu().numpy(), want.astype(np.float16)), (high, low)
 
 
+@pytest.mark.parametrize("cols,rows", [(2080, 1048582), (2083, 1048581)])
+def test_offsets_beyond_32_bits(hom, pkg, cuda, cols, rows):
+    """More than 2^31 values.  They are codes times one, with a largest value of each block between 4 and 6: they come
+    back as they were, and so does their product with the identity, plus themselves."""
+    import torch
+
+    rng = np.random.default_rng(31)
+    grid = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=np.float16)
+    part = grid[rng.integers(0, 8, (4099, cols))] * rng.choice([-1, 1], (4099, cols)).astype(np.float16)
+    part[:, ::32] = grid[rng.integers(6, 8, part[:, ::32].shape)]
+    part = to_dev(part, cuda)
+    x = part.repeat(-(-rows // 4099), 1)[:rows]
+    assert x.numel() > 2 ** 31 and x.is_contiguous()
+
+    def coded(n):
+        return [torch.empty(s, dtype=torch.uint8, device=cuda) for s in pkg.mxf4_shapes(n, cols)]
+
+    q, eye, out = coded(rows), coded(cols), torch.empty_like(x)
+    hom.homQuantizeMxF4F16(x, *q)
+    hom.homDequantizeMxF4F16(*q, out)
+    hom.synchronize()
+    assert torch.equal(out, x)
+    hom.homQuantizeMxF4F16(torch.eye(cols, dtype=torch.float16, device=cuda), *eye)
+    out.fill_(7.0)
+    hom.homGemmMxF4F16(*q, *eye, None, out)
+    hom.synchronize()
+    assert torch.equal(out, x)
+    hom.homGemmMxF4F16(*q, *eye, out, out, beta=1.0)
+    hom.synchronize()
+    assert torch.equal(out, x * 2)
+    turned = x.t().contiguous()
+    del out, x
+    again = coded(rows)
+    hom.homQuantizeMxF4F16(turned, *again, True)
+    hom.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(q, again))
+
+
 def test_streams_graphs_and_declared_weights(hom, pkg, cuda):
     """The same calls eagerly, on another stream, and replayed from two graphs whose replays alternate; the weight is
     quantised into its buffers by the stream itself."""
