@@ -111,6 +111,11 @@ struct Eight<__half> {
     for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
   }
   __device__ __forceinline__ void clear() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void keep(int n) {  // the first n values, zeros behind them
+    uint32_t *word = reinterpret_cast<uint32_t *>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) word[i] = 2 * i + 1 < n ? word[i] : 2 * i < n ? word[i] & 0xffffu : 0u;
+  }
   __device__ __forceinline__ uint32_t largest() const {
     const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
     const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
@@ -154,22 +159,51 @@ struct Eight<float> {
   }
 };
 
+// Eight fp16 values that lie `shift` elements after a 16-byte boundary, in the two 16-byte pieces
+// from there on.
+struct ShiftedEight {
+  uint32_t word[8];
+  __device__ __forceinline__ void load(const uint4 *p) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 piece = p[h];
+      word[4 * h] = piece.x, word[4 * h + 1] = piece.y, word[4 * h + 2] = piece.z, word[4 * h + 3] = piece.w;
+    }
+  }
+  __device__ __forceinline__ Eight<__half> down(int shift) {
+    if (shift & 4)
+#pragma unroll
+      for (int i = 0; i < 6; ++i) word[i] = word[i + 2];
+    if (shift & 2)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) word[i] = word[i + 1];
+    if (shift & 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word[i] = __funnelshift_r(word[i], word[i + 1], 16);
+    Eight<__half> v;
+    v.raw = make_uint4(word[0], word[1], word[2], word[3]);
+    return v;
+  }
+};
+
 // One warp converts a segment of 256 columns of the rows r, r + 32, r + 64 and r + 96 of a
 // 128-row group: four independent loads in flight, and the scales of the four rows are the 16
 // consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED: rows
-// start on 16 bytes (cols % 8 == 0); otherwise the warp reads element by element, coalesced, and
-// sorts the values through shared memory.  (Slower: a persistent form that requests the next unit's
-// values early, whose registers cost more loads in flight than it gains; fp32 values of ragged rows
-// by 4-byte asynchronous copies, 20011 x 777 of them in 19.6 us instead of 16.6.)
+// start on 16 bytes (cols % 8 == 0).  Otherwise, fp16: a lane reads the two 16-byte pieces that its
+// values lie in and moves them down, 20011 x 777 values 15.7 us, 37.9 element by element.  fp32: the
+// warp reads element by element, coalesced, and sorts the values through shared memory, 16.9 us; in
+// 16-byte pieces 24.5, and by 4-byte asynchronous copies 19.6.  (Slower too: a persistent form that
+// requests the next unit's values early, whose registers cost more loads in flight than it gains.)
 //
 // What the rows kernel needs is many loads in flight, so its registers are held down: 65536 x 4096
 // fp16 values 119 us with room for five CTAs on an SM, 112 for eight (6.0 TB/s); 20011 x 776 fp32
 // values 13.0 with five, 13.5 with six, 26 (spills) with eight.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kWarps, sizeof(T) == 2 && ALIGNED ? 8 : 5)
+__global__ void __launch_bounds__(32 * kWarps, sizeof(T) == 2 ? (ALIGNED ? 8 : 5) : 5)
 quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks,
                      uint32_t segments, long long units) {
-  __shared__ __align__(16) T sorted[ALIGNED ? 1 : kWarps][ALIGNED ? 8 : kSegment];
+  constexpr bool kShifted = !ALIGNED && sizeof(T) == 2, kSorted = !ALIGNED && sizeof(T) == 4;
+  __shared__ __align__(16) T sorted[kSorted ? kWarps : 1][kSorted ? kSegment : 8];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -183,17 +217,33 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
   const int col = segment * kSegment + lane * kLaneValues;
 
   Eight<T> v[4];
+  ShiftedEight pieces[kShifted ? 4 : 1];
+  bool whole = false;  // kShifted: the pieces of all rows lie inside the matrix
+  int shift = 0;       // the same for all four rows, which are 32 rows apart
+  if constexpr (kShifted) {
+    const long long begin = row0 * cols + segment * kSegment;
+    const long long last = begin + min(3LL, (rows - 1 - row0) / kRowStep) * kRowStep * cols;
+    whole = row0 < rows && begin >= 8 && last + kSegment + 8 <= rows * cols;
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(x + begin) / 2) & 7;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const long long row = row0 + i * kRowStep;
-    if (ALIGNED) {
+    if constexpr (ALIGNED) {
       if (row < rows && col < cols) v[i].load(x + row * cols + col);
       else v[i].clear();
+    } else if (kShifted && whole) {
+      if (row < rows && col < cols) {
+        pieces[i].load(reinterpret_cast<const uint4 *>(x + row * cols + col - shift));
+      } else {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) pieces[i].word[w] = 0;
+      }
     } else {
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int c = segment * kSegment + j * 32 + lane;
+        const int c = kShifted ? col + j : segment * kSegment + j * 32 + lane;
         w[j] = row < rows && c < cols ? to_float(x[row * cols + c]) : 0.f;
       }
       v[i].set(w);
@@ -202,7 +252,7 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
   uint32_t words[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (!ALIGNED) {
+    if (kSorted) {
       // value j * 32 + lane of the segment in slot j of the lane -> eight consecutive ones
       const T *mine = reinterpret_cast<const T *>(&v[i]);
 #pragma unroll
@@ -210,6 +260,12 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
       __syncwarp();
       v[i].load(&sorted[warp][lane * kLaneValues]);
       __syncwarp();
+    }
+    if constexpr (kShifted) {
+      if (whole) {
+        v[i] = pieces[i].down(shift);
+        if (cols - col < kLaneValues) v[i].keep(cols - col);
+      }
     }
     uint32_t bits = v[i].largest();
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));

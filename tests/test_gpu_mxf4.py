@@ -42,7 +42,7 @@ def _awkward(rng, rows, cols, dtype):
 
 
 SHAPES = [(1, 1), (1, 32), (3, 31), (5, 33), (33, 96), (127, 256), (128, 264), (129, 257), (70, 1000), (260, 513),
-          (4, 4099)]
+          (4, 4099), (300, 1003), (389, 2050)]
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
