@@ -315,12 +315,13 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     if (rank == 0 && elect_one()) {
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
-      int it = 0;
+      int it = 0, n_block = first % p.n_blocks;  // (where A is resident)
       for (int tile = first; tile < last && ok; tile += stride, ++it) {
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + (acc ? kSecondAcc : 0);
-        const bool new_a = resident && (tile == first || tile % p.n_blocks == 0);
-        const bool ends_a = resident && (tile + 1 == last || (tile + 1) % p.n_blocks == 0);
+        const bool new_a = resident && (tile == first || n_block == 0);
+        if (++n_block == p.n_blocks) n_block = 0;
+        const bool ends_a = resident && (tile + 1 == last || n_block == 0);
         for (int i = 0; i < p.steps; ++i) {
           ok = mbar_wait(full_bar(slot), ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (ok && new_a) ok = mbar_wait(a_full_bar(i), a_ph, abort_flag, p.status, kDevWaitTimeoutMma);
@@ -381,22 +382,31 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
     };
     // two neighbouring values of the row of C, requested one tile ahead
-    auto load_row = [&](int tile) {
-      const int col = tile % p.n_blocks * BN + group * 64 + 2 * lane;
+    auto load_row = [&](int n_block) {
+      const int col = n_block * BN + group * 64 + 2 * lane;
       if (ragged) {
         const unsigned short *at = reinterpret_cast<const unsigned short *>(p.C) + col;
         const uint32_t lo = col < p.N ? at[0] : 0u, hi = col + 1 < p.N ? at[1] : 0u;
         return lo | hi << 16;
       }
-      return col < p.N ? *reinterpret_cast<const uint32_t *>(p.C + col) : 0u;
+      return p.C != nullptr && col < p.N ? *reinterpret_cast<const uint32_t *>(p.C + col) : 0u;
     };
     pdl_wait();  // C may be produced, and D still read, by the previous kernel
-    uint32_t next_row = row && first < last ? load_row(first) : 0u;
+    // the tile's place, carried along: a division per tile stood in the way of its first steps
+    int m_block = first / p.n_blocks, n_block = first - m_block * p.n_blocks;
+    const int m_stride = stride / p.n_blocks, n_stride = stride - m_stride * p.n_blocks;
+    uint32_t next_row = row && first < last ? load_row(n_block) : 0u;
     int it = 0;
     for (int tile = first; tile < last; tile += stride, ++it) {
       const int acc = it & 1;
-      const int row0 = tile / p.n_blocks * BM + static_cast<int>(rank) * kHalf + quarter * 32;
-      const int c0 = tile % p.n_blocks * BN + group * 64;
+      const int row0 = m_block * BM + static_cast<int>(rank) * kHalf + quarter * 32;
+      const int c0 = n_block * BN + group * 64;
+      m_block += m_stride;
+      n_block += n_stride;
+      if (n_block >= p.n_blocks) {
+        n_block -= p.n_blocks;
+        ++m_block;
+      }
       // The staging tile was handed to TMA by this warp's previous block: that read must be over
       // before the tile is written again.
       if (ragged) {
@@ -408,34 +418,32 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         mbar_arrive_expect_tx(c_bar(drain), gemm::kEpilogueTileBytes);
         tma_load_2d(stage_smem, &tmC, c_bar(drain), c0, row0);
       }
-      if (row) {
-        __syncwarp();
-        if (general(FORM)) {
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "r"(next_row) : "memory");
-        } else {
-          const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&next_row));
-          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(bias + 8 * lane), "f"(two.x), "f"(two.y) : "memory");
-        }
-        __syncwarp();
-        if (tile + stride < last) next_row = load_row(tile + stride);
-      }
       bool ok = mbar_wait(acc_full_bar(acc), (it >> 1) & 1, abort_flag, p.status, kDevWaitTimeoutEpilogue);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? kSecondAcc : 0) + group * 64;
+      // (not before the wait for the accumulator, where the way to the shared columns would be longer)
+      auto prepare = [&]() {
+        if (row) {
+          if (general(FORM)) {
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(bias + 4 * lane), "r"(next_row) : "memory");
+          } else {
+            const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&next_row));
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(bias + 8 * lane), "f"(two.x), "f"(two.y) : "memory");
+          }
+          if (tile + stride < last) next_row = load_row(n_block);
+        }
+        if (!full && !ragged && lane == 0) bulk_wait_group_read_0();
+        __syncwarp();
+      };
       auto drained = [&]() {
         tc_fence_before_sync();
         __syncwarp();
       };
       auto staging_ready = [&]() {
-        if (ragged) return;
-        if (!full) {
-          if (lane == 0) bulk_wait_group_read_0();
-          __syncwarp();
-        } else {
+        if (full && !ragged)
           ok = __all_sync(0xffffffffu, mbar_wait(c_bar(drain), it & 1, abort_flag, p.status, kDevWaitTimeoutEpilogue));
-        }
       };
       if (acc ? group < kSharingGroups : group >= 4 - kSharingGroups) {
         uint32_t lo[32], hi[32];
@@ -445,12 +453,14 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         drained();
         arrive_even(shared_bar);
         arrive_even(acc_empty_bar(acc));
+        prepare();
         staging_ready();
         finish_half<FORM>(p, lo, 0, my_row, bias, lane);
         finish_half<FORM>(p, hi, 1, my_row, bias, lane);
       } else {
         uint32_t v[32];
         tmem_ld_32x32(t_row, v);
+        prepare();
         tmem_ld_wait();
         staging_ready();
         finish_half<FORM>(p, v, 0, my_row, bias, lane);
@@ -492,12 +502,14 @@ using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUte
 
 bool run_product_pair(const Problem &pb, cudaStream_t stream) {
   static const Kernel kernels[] = {gemm_mxf4_pair_kernel<kNone>,        gemm_mxf4_pair_kernel<kRow>,
-                                   gemm_mxf4_pair_kernel<kFull>,        gemm_mxf4_pair_kernel<kGelu>,
-                                   gemm_mxf4_pair_kernel<kRow | kGelu>, gemm_mxf4_pair_kernel<kFull | kGelu>,
-                                   gemm_mxf4_pair_kernel<kAny>,          gemm_mxf4_pair_kernel<kRagged>};
+                                   gemm_mxf4_pair_kernel<kFull>,        gemm_mxf4_pair_kernel<kRow | kGelu>,
+                                   gemm_mxf4_pair_kernel<kFull | kGelu>, gemm_mxf4_pair_kernel<kAny>,
+                                   gemm_mxf4_pair_kernel<kRagged>};
   const bool units = pb.alpha == 1.f && (pb.c_mode == 0 || pb.beta == 1.f);
   const bool ragged = pb.N % 8 != 0;
-  const Kernel kernel = kernels[ragged ? 7 : !units ? 6 : (pb.act ? 3 : 0) + (pb.c_mode == 0 ? 0 : pb.c_mode == 2 ? 1 : 2)];
+  // GELU without C runs as with a row of zeros: without the reads between them, its steps were taken up
+  // before the shared columns were given back (32768 x 4096 x 1024 111 us, with the zeros 96).
+  const Kernel kernel = kernels[ragged ? 6 : !units ? 5 : pb.act ? (pb.c_mode == 1 ? 4 : 3) : pb.c_mode == 0 ? 0 : pb.c_mode == 2 ? 1 : 2];
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
