@@ -17,7 +17,12 @@
 // of scales: the first lies in [0, 256), the second in [160, 416), and the warps that drain the 96
 // columns they share take them into registers at once, so that the next tile's MMAs can start while
 // the rest is drained beside them.  (192-column tiles need not share, but pull 13 % more through L2
-// for the same work: 16384 x 4096 x 4096 120 us, 32768 x 4096 x 1024 73 instead of 69.)
+// for the same work: 16384 x 4096 x 4096 120 us instead of 107, 32768 x 4096 x 1024 73 instead of 69.)
+//
+// With GELU the epilogue's instructions are the bound where K is small: 131072 x 4096 x 256 takes
+// 277 us, 209 without GELU, the rate at which D can be written; 3400 of the 5300 cycles that a tile
+// takes are arithmetic.  What lies between two tiles' arithmetic counts as well: with a division for
+// the tile's place, and the row of C laid out before the accumulator was asked for, 293 us.
 //
 //   warps 0, 2, 3  TMA producers of A's codes, of B's and of the scales
 //   warp 1         tensor memory, scale copies and MMA issue (even CTA)
@@ -574,9 +579,9 @@ bool run_product_pair(const Problem &pb, cudaStream_t stream) {
   p.tiles = static_cast<int>(tiles);
   if (p.tiles < pairs) pairs = p.tiles;
   // Keeping A saves half of what is pulled through L2, but lets the pairs drift apart; measured with
-  // and without, in us: 32768 x 4096 x 1024 68 / 74, 131072 x 4096 x 1024 with GELU and a row of C
-  // 343 / 352, 32768 x 2304 x 768 38.8 / 40.6; with a matrix C, whose tiles are read as well,
-  // 16384 x 4096 x 1024 54.5 / 53.1, 32768 x 1024 x 1024 31.0 / 29.6, 32768 x 768 x 768 25.8 / 24.3.
+  // and without, in us: 32768 x 4096 x 1024 68 / 76, 131072 x 4096 x 1024 with GELU and a row of C
+  // 338 / 359, 32768 x 2304 x 768 41.0 / 43.2; with a matrix C, whose tiles are read as well,
+  // 16384 x 4096 x 1024 55.3 / 54.2, 32768 x 1024 x 1024 32.4 / 31.4, 32768 x 768 x 768 26.3 / 25.9.
   p.resident = p.steps <= kStages && p.tiles >= 2 * pairs && pb.c_mode != 1 ? 1 : 0;
 
   cfg.gridDim = dim3(2 * pairs);
