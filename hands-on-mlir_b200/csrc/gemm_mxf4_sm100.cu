@@ -18,6 +18,7 @@
 //   warp 0  TMA producer      warp 1  tensor memory, scale copies, MMA issue
 //   warps 2-9  accumulator exchange and epilogue
 #include <atomic>
+#include <type_traits>
 
 #include "gemm_sm100.cuh"
 #include "mxf4_epilogue.cuh"
@@ -68,15 +69,22 @@ __device__ __forceinline__ uint32_t cluster_nctas() {
   return r;
 }
 
-__device__ __forceinline__ float2 epilogue2(const Params &p, float2 v, float2 c) {
-  v = __fmul2_rn(make_float2(p.alpha, p.alpha), v);
-  if (p.c_mode != 0) v = __ffma2_rn(make_float2(p.beta, p.beta), c, v);
-  if (p.act == 1) {
-    float2 x[1] = {v};
-    gelu2(x);
-    return x[0];
+// Where a row of the exchanged tile has its 16-byte chunk: neither the stores (a chunk of 32 rows) nor
+// the loads (every other chunk of a row, first the even, then the odd ones) meet in a bank.
+__device__ __forceinline__ uint32_t place_of(int chunk, int row) {
+  return static_cast<uint32_t>(chunk ^ (row & 7) ^ (chunk >> 3));
+}
+
+// Of PAIRS pairs of sums and of C's values.  All of them take each step together: one test of `act`
+// with one copy of its code behind it, and the rest in a straight line.
+template <int PAIRS>
+__device__ __forceinline__ void epilogue2(const Params &p, float2 (&v)[PAIRS], const float2 (&c)[PAIRS]) {
+#pragma unroll
+  for (int i = 0; i < PAIRS; ++i) {
+    v[i] = __fmul2_rn(make_float2(p.alpha, p.alpha), v[i]);
+    if (p.c_mode != 0) v[i] = __ffma2_rn(make_float2(p.beta, p.beta), c[i], v[i]);
   }
-  return v;
+  if (p.act == 1) gelu2(v);
 }
 
 // ALIGNED: N % 8 == 0, rows of C and D travel in 16-byte pieces; otherwise element by element,
@@ -127,8 +135,10 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();
   // Cluster barrier, phase 1: "this CTA runs"; its shared memory may be written by its peers.
-  // Every thread of every CTA arrives and waits exactly once per phase, on error paths too.
-  cluster_arrive();
+  // Every thread of every CTA arrives and waits exactly once per phase, on error paths too.  (A CTA
+  // that has the tile to itself does without: its parts go from warp to warp.)
+  const bool alone = parts == 1;
+  if (!alone) cluster_arrive();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -170,9 +180,11 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
     __syncwarp();
-    cluster_wait();
-    cluster_arrive();
-    cluster_wait();
+    if (!alone) {
+      cluster_wait();
+      cluster_arrive();
+      cluster_wait();
+    }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issuer
     if (elect_one()) {
@@ -200,9 +212,11 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (ok) tc_commit(acc_bar);
     }
     __syncwarp();
-    cluster_wait();
-    cluster_arrive();
-    cluster_wait();
+    if (!alone) {
+      cluster_wait();
+      cluster_arrive();
+      cluster_wait();
+    }
   } else {
     // ------------------------------------------- accumulator exchange and epilogue
     const int rows = min(BM, p.M - m0);               // rows of the tile inside the matrix
@@ -211,7 +225,9 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int my_rows = max(0, min(rows_per, rows - row_first));
     const int t = threadIdx.x - 64;
     constexpr int kPieces = BN / 8;  // 8-column pieces of an output row
-    constexpr int kTasks = ALIGNED ? BM * kPieces / kExchangeThreads : 1;
+    constexpr int kPieceRows = kExchangeThreads / kPieces;  // 32 rows of pieces at a time
+    constexpr int kTasks = ALIGNED ? BM / kPieceRows : 1;
+    static_assert(kPieceRows == 32 && kPieceRows / (kExchangeThreads / 32) == 4, "four rows to a warp, four times");
     // not aligned: one column per thread and every fourth row, a batch of them at a time; C's values of
     // the first batch are asked for now, like the pieces above
     constexpr int kRowStep = kExchangeThreads / BN, kRows = 16;
@@ -244,7 +260,7 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
     bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, kDevWaitTimeoutEpilogue);
     ok = __all_sync(0xffffffffu, ok);
-    cluster_wait();  // phase 1: every CTA of the cluster runs
+    if (!alone) cluster_wait();  // phase 1: every CTA of the cluster runs
     if (ok) {
       tc_fence_after_sync();
       const int quarter = warp & 3;
@@ -263,8 +279,7 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (row < rows) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              // 16-byte chunks of a row are XOR-swizzled by the row: conflict-free stores
-              const uint32_t chunk = static_cast<uint32_t>((col_begin + h * 32) / 4 + j) ^ (local & 7);
+              const uint32_t chunk = place_of((col_begin + h * 32) / 4 + j, local);
               asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + chunk * 16), "r"(acc[4 * j]),
                            "r"(acc[4 * j + 1]), "r"(acc[4 * j + 2]), "r"(acc[4 * j + 3])
                            : "memory");
@@ -274,44 +289,59 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         tc_fence_before_sync();
       }
     }
-    cluster_arrive();  // phase 2: the parts are delivered
-    cluster_wait();
+    if (alone) {
+      asm volatile("bar.sync 1, %0;" ::"n"(kExchangeThreads) : "memory");
+    } else {
+      cluster_arrive();  // phase 2: the parts are delivered
+      cluster_wait();
+    }
     if (ok) {
-      // the sum of the parts, in part order, at (local row, chunk of four columns)
-      auto total = [&](int local, int chunk) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q = 0; q < parts; ++q) {
-          float4 f;
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
-                       : "r"(smem_base + kRecv + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
-                             (static_cast<uint32_t>(chunk) ^ (local & 7)) * 16)
-                       : "memory");
-          v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
-        }
-        return v;
-      };
+      // the sums of the parts, in part order
       if constexpr (ALIGNED) {
+        const int piece = t % kPieces, col = n0 + piece * 8;
+        auto finish = [&](auto count) {  // of the pieces that this thread may have
+          constexpr int kCount = decltype(count)::value;
+          float2 v[kCount * 4], c[kCount * 4];
 #pragma unroll
-        for (int i = 0; i < kTasks; ++i) {
-          const int local = (t + i * kExchangeThreads) / kPieces, piece = (t + i * kExchangeThreads) % kPieces;
-          const int col = n0 + piece * 8;
-          if (local < my_rows && col < p.N) {
-            const __half2 *c2 = reinterpret_cast<const __half2 *>(&cval[i]);
+          for (int i = 0; i < kCount * 4; ++i) {
+            v[i] = make_float2(0.f, 0.f);
+            c[i] = __half22float2(reinterpret_cast<const __half2 *>(&cval[i / 4])[i % 4]);
+          }
+          for (int q = 0; q < parts; ++q) {
+            float f[kCount * 8];
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+              const int local = min(t / kPieces + i * kPieceRows, rows_per - 1);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(f[8 * i + 4 * h]), "=f"(f[8 * i + 4 * h + 1]), "=f"(f[8 * i + 4 * h + 2]),
+                               "=f"(f[8 * i + 4 * h + 3])
+                             : "r"(smem_base + kRecv + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
+                                   place_of(2 * piece + h, local) * 16)
+                             : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < kCount * 4; ++i) v[i] = __fadd2_rn(v[i], make_float2(f[2 * i], f[2 * i + 1]));
+          }
+          epilogue2(p, v, c);
+#pragma unroll
+          for (int i = 0; i < kCount; ++i) {
+            const int local = t / kPieces + i * kPieceRows;
             uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float4 v = total(local, 2 * piece + j);
-              const float2 x = epilogue2(p, make_float2(v.x, v.y), __half22float2(c2[2 * j]));
-              const float2 y = epilogue2(p, make_float2(v.z, v.w), __half22float2(c2[2 * j + 1]));
-              const __half2 hx = __floats2half2_rn(x.x, x.y), hy = __floats2half2_rn(y.x, y.y);
-              w[2 * j] = *reinterpret_cast<const uint32_t *>(&hx);
-              w[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&hy);
+            for (int j = 0; j < 4; ++j) {
+              const __half2 h = __floats2half2_rn(v[4 * i + j].x, v[4 * i + j].y);
+              w[j] = *reinterpret_cast<const uint32_t *>(&h);
             }
-            *reinterpret_cast<uint4 *>(p.D + static_cast<long long>(m0 + row_first + local) * p.N + col) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            if (local < my_rows && col < p.N)
+              *reinterpret_cast<uint4 *>(p.D + static_cast<long long>(m0 + row_first + local) * p.N + col) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
           }
-        }
+        };
+        if (rows_per > 2 * kPieceRows) finish(std::integral_constant<int, 4>());
+        else if (rows_per > kPieceRows) finish(std::integral_constant<int, 2>());
+        else if (warp - 2 < (my_rows + 3) / 4) finish(std::integral_constant<int, 1>());
       } else {
         const uint32_t at = smem_base + kRecv + (column & 3) * 4;
         for (int base = t / BN; base < my_rows; base += kRows * kRowStep) {
@@ -327,17 +357,22 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               asm volatile("ld.shared.f32 %0, [%1];"
                            : "=f"(f[i])
                            : "r"(at + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
-                                 (static_cast<uint32_t>(column >> 2) ^ (local & 7)) * 16));
+                                 place_of(column >> 2, local) * 16));
             }
 #pragma unroll
             for (int i = 0; i < kRows; ++i) v[i] += f[i];
           }
+          float2 pair[kRows / 2], c[kRows / 2];
+#pragma unroll
+          for (int i = 0; i < kRows / 2; ++i) {
+            pair[i] = make_float2(v[2 * i], v[2 * i + 1]);
+            c[i] = make_float2(__half2float(__ushort_as_half(c_bits[2 * i])), __half2float(__ushort_as_half(c_bits[2 * i + 1])));
+          }
+          epilogue2(p, pair, c);
           __half *d = p.D + static_cast<long long>(m0 + row_first + base) * p.N + col;
 #pragma unroll
           for (int i = 0; i < kRows; ++i) {
-            const float2 r = epilogue2(p, make_float2(v[i], 0.f),
-                                       make_float2(__half2float(__ushort_as_half(c_bits[i])), 0.f));
-            if (base + i * kRowStep < my_rows && col < p.N) *d = __float2half_rn(r.x);
+            if (base + i * kRowStep < my_rows && col < p.N) *d = __float2half_rn(i & 1 ? pair[i / 2].y : pair[i / 2].x);
             d += static_cast<long long>(kRowStep) * p.N;
           }
         }
