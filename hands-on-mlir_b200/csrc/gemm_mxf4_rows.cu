@@ -3,9 +3,9 @@
 // does without tensor memory, TMA and barriers: a warp takes a row of B, a lane one block of 32
 // values out of 32 (16 bytes, a warp 512 contiguous ones).
 //
-// Measured per call in a chain of calls, against the tensor-core kernel (us): one row of 1024 values
-// by 4096 columns with a row of C and GELU 2.7 / 7.1, of 768 by 768 1.6 / 3.2, two rows of 1024 by
-// 4096 2.5 / 4.6; with four rows the two are even.  Two or four rows of B for a warp were slower.
+// Measured per call in a chain of calls, against the tensor-core kernel (us): one row of 768 values by
+// 768 columns 1.9 / 2.7, two rows of 1024 by 4096 2.7 / 3.5.  The tensor-core kernel's time does not
+// grow with the rows, this one's does.  Two or four rows of B for a warp were slower.
 //
 // Arithmetic is exact until the blocks are added: a product of two codes is at most 36 in quarters,
 // so eight of them add up to at most 1152 quarters, which fp16 holds exactly (11 bits); the four

@@ -2,9 +2,10 @@
 // path, for problems with few output tiles: D = act(alpha * A.B^T + beta * C), fp32 accumulation,
 // fp16 C and D.  And the choice between this form and the others.
 //
-// A 128 x 64 tile of D belongs to a cluster of one, two or four CTAs that share its K range.  A K step is 256 values: 128 bytes of codes a row, fetched by TMA into 128-byte-swizzled
-// tiles like the fp16 kernels' 64 values, and two scale tiles for each operand, which tcgen05.cp
-// takes from shared to tensor memory right before the four MMAs that use them.  Zeros that TMA fills
+// A 128 x 64 tile of D belongs to a cluster of one, two or four CTAs that share its K range.  A K
+// step is 256 values: 128 bytes of codes a row, fetched by TMA into 128-byte-swizzled tiles like the
+// fp16 kernels' 64 values, and two scale tiles for each operand, which tcgen05.cp takes from shared
+// to tensor memory right before the four MMAs that use them.  Zeros that TMA fills
 // in beyond the matrix (codes 0, scales 2^-127) add nothing.  A stage of the ring has scales of its
 // own in tensor memory: that the stage was filled again says that the MMAs of its last use, and
 // their reads of the scales, are over.
@@ -12,8 +13,14 @@
 // The partial tiles are exchanged SM to SM as in the fp16 cluster kernel (gemm_cluster_sm100.cu):
 // CTA r owns rows [r, r + 1) * ceil(rows / parts) of the tile, every CTA stores its part of them
 // into the owner's shared memory, and after a cluster barrier the owner adds the parts in part order
-// (bit-identical from run to run), applies the epilogue and writes full rows.  What bounds it is
-// latency: launch, first loads, exchange and store one after the other.
+// (bit-identical from run to run), applies the epilogue and writes full rows.  A CTA that has its tile
+// to itself passes it through its shared memory the same way, to write full rows.
+//
+// What bounds it is latency: launch, first loads, exchange and store one after the other.  128 x 768
+// x 768 takes 5900 cycles from entry to exit: 1500 until the previous kernel is waited for, 2400 for
+// the first loads and three steps, 800 to take the accumulator to shared memory, 1200 for sums,
+// epilogue and stores.  (With a branch, a loop and a copy of the GELU for every piece of eight values
+// the last were 3400.)  A further step takes 0.2 us, the rate at which L2 feeds one SM.
 //
 //   warp 0  TMA producer      warp 1  tensor memory, scale copies, MMA issue
 //   warps 2-9  accumulator exchange and epilogue
@@ -39,7 +46,6 @@ constexpr int kStepTiles = kStepBlocks / kTileBlocks;  // 2 scale tiles
 constexpr int kStages = 4;
 constexpr int kExchangeThreads = 256;
 constexpr int kThreads = 64 + kExchangeThreads;
-constexpr int kMaxParts = 4;
 constexpr uint32_t kABytes = BM * kStepBytes, kBBytes = BN * kStepBytes;
 constexpr uint32_t kScaleBytes = kStepTiles * kTileBytes;
 constexpr uint32_t kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
@@ -432,18 +438,22 @@ bool launch(const Problem &pb, int parts, cudaStream_t stream) {
 }  // namespace
 
 // Measured per call in a chain of calls (us):
-//   one wave of 128 x 64 tiles against the pairs' 256 x 256: 1024 x 1024 x 1024 5.5 / 5.7,
-//   1024 x 1024 x 4096 7.9 / 9.4, 512 x 2304 x 768 5.5 / 5.5; more than one wave: 512 x 4096 x 1024
-//   10.7 / 5.8, 2048 x 1024 x 1024 10.6 / 5.9;
-//   K in one, two and four parts: 64 x 1024 x 4096 6.6 / 4.8 / 4.6, 128 x 4096 x 4096 7.5 / 6.4 / 12.5
-//   (the last no longer in one wave), 128 x 1024 x 1024 5.0 / 4.6 / 4.8, 385 x 1001 x 808 9.6 / 7.5.
+//   one wave of 128 x 64 tiles against the pairs' 256 x 256: 1024 x 1024 x 1024 3.7 / 5.7,
+//   1024 x 1024 x 4096 6.1 / 9.3, 512 x 2304 x 768 3.6 / 5.5; more than one wave: 2048 x 768 x 768
+//   6.5 / 5.4, 512 x 4096 x 1024 7.2 / 5.8;
+//   K in one, two and four parts, 128 rows: 1024 columns and K = 1024 3.3 / 3.8 / 4.1, 2560 4.4 / 4.3 /
+//   4.5, 4096 5.6 / 4.9 / 4.7, 8192 8.8 / 6.5 / 5.4; 1792 columns and K = 4096 5.6 / 5.0 / 5.4, 4096
+//   columns 5.7 / 5.6 / 11.2 (the last no longer in one wave: clusters of four need SMs of one GPC);
+//   32 rows, which are little to exchange, 256 columns and K = 1536 3.2 / 3.1 / 3.1, 2048 3.6 / 3.3 / 3.1.
 bool run_product(const Problem &pb, cudaStream_t stream) {
   if (pb.M <= kMaxFewRows) return run_product_rows(pb, stream);
   const int64_t tiles = (pb.M + BM - 1) / BM * ((pb.N + BN - 1) / BN), sms = sm_count();
   if (tiles > sms) return run_product_pair(pb, stream);
   const int64_t steps = (pb.blocks + kStepBlocks - 1) / kStepBlocks;
-  // (clusters of four need SMs of one GPC: not quite all of the chip can be had)
-  const int parts = steps >= 8 && tiles * kMaxParts <= sms - sms / 8 ? kMaxParts : steps >= 4 && 2 * tiles <= sms ? 2 : 1;
+  const bool few_rows = pb.M <= 32;
+  int parts = 1;
+  if (2 * tiles <= sms && steps >= (few_rows ? 6 : 3 * tiles <= sms ? 10 : 16)) parts = 2;
+  if (8 * tiles <= sms && steps >= (few_rows ? 8 : 12)) parts = 4;
   return pb.N % 8 == 0 ? launch<true>(pb, parts, stream) : launch<false>(pb, parts, stream);
 }
 

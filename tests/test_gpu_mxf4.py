@@ -134,7 +134,8 @@ def _product(hom, cuda, a, sa, b, sb, c, d, act=0, alpha=1.0, beta=0.0):
 PRODUCTS = [(1, 8, 32), (1, 4096, 1024), (2, 1, 32), (2, 333, 5000), (7, 33, 96), (16, 768, 4096), (33, 77, 2100),
             (127, 129, 256), (128, 128, 288), (129, 200, 544), (385, 1001, 808), (300, 1000, 800), (640, 512, 1056),
             (1100, 2304, 768), (2500, 1024, 520), (1001, 2001, 1060), (3900, 2400, 300), (4001, 2391, 600),
-            (5, 72, 40000), (900, 1288, 2500)]
+            (5, 72, 40000), (900, 1288, 2500), (100, 1001, 3000), (130, 1000, 2600), (128, 4000, 4200), (200, 777, 4100),
+            (20, 640, 1700)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
