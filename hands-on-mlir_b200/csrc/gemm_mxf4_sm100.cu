@@ -94,7 +94,9 @@ __device__ __forceinline__ void epilogue2(const Params &p, float2 (&v)[PAIRS], c
 }
 
 // ALIGNED: N % 8 == 0, rows of C and D travel in 16-byte pieces; otherwise element by element,
-// neighbouring threads at neighbouring columns.
+// neighbouring threads at neighbouring columns.  (Two columns a lane, as one where the row's address
+// allows it: the choice between two kinds of load keeps them from being under way together, 385 x
+// 1001 x 808 7.1 us.)
 template <bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -234,21 +236,10 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     constexpr int kPieceRows = kExchangeThreads / kPieces;  // 32 rows of pieces at a time
     constexpr int kTasks = ALIGNED ? BM / kPieceRows : 1;
     static_assert(kPieceRows == 32 && kPieceRows / (kExchangeThreads / 32) == 4, "four rows to a warp, four times");
-    // not aligned: one column per thread and every fourth row, a batch of them at a time; C's values of
-    // the first batch are asked for now, like the pieces above
-    constexpr int kRowStep = kExchangeThreads / BN, kRows = 16;
-    const int column = t % BN, col = n0 + column;
+    // not aligned: one column per thread and every fourth row
+    constexpr int kRowStep = kExchangeThreads / BN, kRows = BM / kRowStep;
+    const int column = t % BN, first_local = t / BN;
     unsigned short c_bits[ALIGNED ? 1 : kRows];
-    auto load_c = [&](int base) {
-      const unsigned short *c = reinterpret_cast<const unsigned short *>(p.C) + col +
-                                (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + base) * p.N : 0);
-      const long long step = p.c_mode == 1 ? static_cast<long long>(kRowStep) * p.N : 0;
-#pragma unroll
-      for (int i = 0; i < (ALIGNED ? 1 : kRows); ++i) {
-        c_bits[i] = p.c_mode != 0 && base + i * kRowStep < my_rows && col < p.N ? *c : 0;
-        c += step;
-      }
-    };
 
     pdl_wait();  // C may be produced, and D still read, by the previous kernel
     uint4 cval[kTasks];
@@ -262,7 +253,15 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               p.C + (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + row) * p.N : 0) + col);
       }
     } else {
-      load_c(t / BN);
+      const int col = n0 + column;
+      const unsigned short *c = reinterpret_cast<const unsigned short *>(p.C) + col +
+                                (p.c_mode == 1 ? static_cast<long long>(m0 + row_first + first_local) * p.N : 0);
+      const long long step = p.c_mode == 1 ? static_cast<long long>(kRowStep) * p.N : 0;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        c_bits[i] = p.c_mode != 0 && first_local + i * kRowStep < my_rows && col < p.N ? *c : 0;
+        c += step;
+      }
     }
     bool ok = mbar_wait(acc_bar, 0, abort_flag, p.status, kDevWaitTimeoutEpilogue);
     ok = __all_sync(0xffffffffu, ok);
@@ -349,39 +348,40 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         else if (rows_per > kPieceRows) finish(std::integral_constant<int, 2>());
         else if (warp - 2 < (my_rows + 3) / 4) finish(std::integral_constant<int, 1>());
       } else {
-        const uint32_t at = smem_base + kRecv + (column & 3) * 4;
-        for (int base = t / BN; base < my_rows; base += kRows * kRowStep) {
-          if (base >= kRowStep) load_c(base);
-          float v[kRows];
+        auto finish = [&](auto count) {
+          constexpr int kCount = decltype(count)::value;
+          float2 v[kCount / 2], c[kCount / 2];  // of two of the thread's rows
 #pragma unroll
-          for (int i = 0; i < kRows; ++i) v[i] = 0.f;
-          for (int q = 0; q < parts; ++q) {
-            float f[kRows];
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-              const int local = min(base + i * kRowStep, my_rows - 1);
-              asm volatile("ld.shared.f32 %0, [%1];"
-                           : "=f"(f[i])
-                           : "r"(at + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
-                                 place_of(column >> 2, local) * 16));
-            }
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) v[i] += f[i];
-          }
-          float2 pair[kRows / 2], c[kRows / 2];
-#pragma unroll
-          for (int i = 0; i < kRows / 2; ++i) {
-            pair[i] = make_float2(v[2 * i], v[2 * i + 1]);
+          for (int i = 0; i < kCount / 2; ++i) {
+            v[i] = make_float2(0.f, 0.f);
             c[i] = make_float2(__half2float(__ushort_as_half(c_bits[2 * i])), __half2float(__ushort_as_half(c_bits[2 * i + 1])));
           }
-          epilogue2(p, pair, c);
-          __half *d = p.D + static_cast<long long>(m0 + row_first + base) * p.N + col;
+          for (int q = 0; q < parts; ++q) {
+            float f[kCount];
 #pragma unroll
-          for (int i = 0; i < kRows; ++i) {
-            if (base + i * kRowStep < my_rows && col < p.N) *d = __float2half_rn(i & 1 ? pair[i / 2].y : pair[i / 2].x);
+            for (int i = 0; i < kCount; ++i) {
+              const int local = min(first_local + i * kRowStep, rows_per - 1);
+              asm volatile("ld.shared.f32 %0, [%1];"
+                           : "=f"(f[i])
+                           : "r"(smem_base + kRecv + static_cast<uint32_t>(q * rows_per + local) * (BN * 4) +
+                                 place_of(column >> 2, local) * 16 + (column & 3) * 4)
+                           : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < kCount / 2; ++i) v[i] = __fadd2_rn(v[i], make_float2(f[2 * i], f[2 * i + 1]));
+          }
+          epilogue2(p, v, c);
+          const int col = n0 + column;
+          __half *d = p.D + static_cast<long long>(m0 + row_first + first_local) * p.N + col;
+#pragma unroll
+          for (int i = 0; i < kCount; ++i) {
+            if (first_local + i * kRowStep < my_rows && col < p.N) *d = __float2half_rn(i & 1 ? v[i / 2].y : v[i / 2].x);
             d += static_cast<long long>(kRowStep) * p.N;
           }
-        }
+        };
+        if (rows_per > BM / 2) finish(std::integral_constant<int, kRows>());
+        else if (rows_per > BM / 4) finish(std::integral_constant<int, kRows / 2>());
+        else finish(std::integral_constant<int, kRows / 4>());
       }
     }
   }
