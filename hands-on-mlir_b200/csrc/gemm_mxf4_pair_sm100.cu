@@ -81,7 +81,9 @@ struct Params {
   int resident;  // steps <= kStages: A's rows stay in shared memory for the tiles of a row block
   int b_early;   // B is a declared constant: request its first tiles before griddepcontrol.wait
   int *status;
+  int fill[6];
 };
+static_assert(quick_to_launch<Params>, "see launch_pdl");  // (the tensor maps before it are whole 64 bytes)
 
 // Which C and activation an instantiation handles, with alpha = beta = 1; kAny handles all of it,
 // kRagged also N that is not a multiple of 8: rows of C and D then start at any element, and the

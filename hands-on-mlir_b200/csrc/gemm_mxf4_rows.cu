@@ -32,6 +32,7 @@ struct Params {
   int n, blocks, tile_cols;
   int b_early;  // B is a declared constant: read before griddepcontrol.wait
 };
+static_assert(quick_to_launch<Params>, "see launch_pdl");
 
 __device__ __forceinline__ void decode32(const uint4 &codes, __half2 (&v)[16]) {
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};

@@ -67,7 +67,9 @@ struct Params {
   int M, N, steps, n_blocks;
   int b_early;  // B is a declared constant: request its tiles before griddepcontrol.wait
   int *status;
+  int fill[8];
 };
+static_assert(quick_to_launch<Params>, "see launch_pdl");  // (the tensor maps before it are whole 64 bytes)
 
 __device__ __forceinline__ uint32_t cluster_nctas() {
   uint32_t r;

@@ -161,6 +161,12 @@ void split_workspace_mark_dirty();
 // as clusters of that many CTAs along x).  Every kernel of this library calls
 // griddepcontrol.wait before its first dependent global-memory access, which is what makes the
 // relaxed launch order safe.
+//
+// What a launch costs the host depends on the size of the kernel's parameters: 1.65 us where they end
+// 17 to 32 bytes after a multiple of 64, 2.1 us elsewhere (measured from 8 to 904 bytes, with and
+// without clusters).  Kernels as short as a launch fill theirs up to such a size.
+template <typename P>
+constexpr bool quick_to_launch = sizeof(P) % 64 > 16 && sizeof(P) % 64 <= 32;
 template <typename... KernelArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, size_t smem,
                               cudaStream_t stream, unsigned cluster_x, Args &&...args) {

@@ -22,6 +22,16 @@ constexpr int kLaneValues = 8;                     // consecutive values of a ro
 constexpr int kSegment = 32 * kLaneValues;         // a warp's part of a row: 8 blocks, 2 scale tiles wide
 constexpr int kRowStep = kTileRows / 4;            // a warp works on rows r, r + 32, r + 64, r + 96
 
+struct Params {
+  const void *values;  // of the matrix that is read or written
+  uint8_t *codes, *scales;
+  long long rows, units;
+  int cols, blocks;
+  uint32_t segments;
+  int fill[9];
+};
+static_assert(quick_to_launch<Params>, "see launch_pdl");
+
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // The scale byte of a block whose largest magnitude has these bits (NaN and infinity compare
@@ -191,7 +201,7 @@ struct ShiftedEight {
 // consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED: rows
 // start on 16 bytes (cols % 8 == 0).  Otherwise, fp16: a lane reads the two 16-byte pieces that its
 // values lie in and moves them down, 20011 x 777 values 15.7 us, 37.9 element by element.  fp32: the
-// warp reads element by element, coalesced, and sorts the values through shared memory, 16.9 us; in
+// warp reads element by element, coalesced, and sorts the values through shared memory, 15.9 us; in
 // 16-byte pieces 24.5, and by 4-byte asynchronous copies 19.6.  (Slower too: a persistent form that
 // requests the next unit's values early, whose registers cost more loads in flight than it gains.)
 //
@@ -200,8 +210,11 @@ struct ShiftedEight {
 // values 13.0 with five, 13.5 with six, 26 (spills) with eight.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kWarps, sizeof(T) == 2 ? (ALIGNED ? 8 : 5) : 5)
-quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks,
-                     uint32_t segments, long long units) {
+quantize_rows_kernel(const Params p) {
+  const T *x = static_cast<const T *>(p.values);
+  const long long rows = p.rows, units = p.units;
+  const int cols = p.cols, blocks = p.blocks;
+  const uint32_t segments = p.segments;
   constexpr bool kShifted = !ALIGNED && sizeof(T) == 2, kSorted = !ALIGNED && sizeof(T) == 4;
   __shared__ __align__(16) T sorted[kSorted ? kWarps : 1][kSorted ? kSegment : 8];
   hom::ptx::pdl_launch_dependents();
@@ -274,7 +287,7 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
     const uint32_t packed = byte == 255u ? 0u : v[i].encode(reciprocal_scale(byte));
     const long long row = row0 + i * kRowStep;
     if (row < rows && col < blocks * kBlock)
-      *reinterpret_cast<uint32_t *>(codes + row * (blocks * 16LL) + col / 2) = packed;
+      *reinterpret_cast<uint32_t *>(p.codes + row * (blocks * 16LL) + col / 2) = packed;
     // the bytes of four neighbouring blocks become the word of one scale tile
     uint32_t word = byte << (8 * ((lane >> 2) & 3));
     word |= __shfl_xor_sync(0xffffffffu, word, 4);
@@ -284,7 +297,7 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
   const int tile_cols = (blocks + kTileBlocks - 1) / kTileBlocks;
   const int tile = segment * 2 + (lane >> 4);
   if ((lane & 15) == 0 && tile < tile_cols)
-    *reinterpret_cast<uint4 *>(scales + (group * tile_cols + tile) * kTileBytes + r * 16) =
+    *reinterpret_cast<uint4 *>(p.scales + (group * tile_cols + tile) * kTileBytes + r * 16) =
         make_uint4(words[0], words[1], words[2], words[3]);
 }
 
@@ -295,7 +308,10 @@ quantize_rows_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows
 // 8 KB), with 2-byte loads 27.7.
 template <typename T, int COLUMNS>
 __global__ void __launch_bounds__(kTileRows * kTileBlocks / COLUMNS)
-quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long rows, int cols, int blocks) {
+quantize_columns_kernel(const Params p) {
+  const T *x = static_cast<const T *>(p.values);
+  const long long rows = p.rows;
+  const int cols = p.cols, blocks = p.blocks;
   __shared__ __align__(16) uint8_t tile_bytes[kTileBytes];
   hom::ptx::pdl_launch_dependents();
   hom::ptx::pdl_wait();
@@ -342,7 +358,7 @@ quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long r
       packed[q] = byte == 255u ? 0u : encode8(part);
     }
     if (row0 < rows && block < blocks)
-      *reinterpret_cast<uint4 *>(codes + ((row0 + c) * blocks + block) * 16) =
+      *reinterpret_cast<uint4 *>(p.codes + ((row0 + c) * blocks + block) * 16) =
           make_uint4(packed[0], packed[1], packed[2], packed[3]);
     const int r = r0 + c;
     tile_bytes[(r & 31) * 16 + (r >> 5) * 4 + b] = static_cast<uint8_t>(byte);
@@ -350,7 +366,7 @@ quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long r
   __syncthreads();
   const int t = static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x);
   if (t < kTileBytes / 16)
-    reinterpret_cast<uint4 *>(scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[t] =
+    reinterpret_cast<uint4 *>(p.scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[t] =
         reinterpret_cast<const uint4 *>(tile_bytes)[t];
 }
 
@@ -359,8 +375,11 @@ quantize_columns_kernel(const T *x, uint8_t *codes, uint8_t *scales, long long r
 // consecutive bytes (20011 x 776 fp32 values: two half-filled stores a lane 16.4 us).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kWarps)
-dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *out,
-                  long long rows, int cols, int blocks, int segments, long long units) {
+dequantize_kernel(const Params p) {
+  T *out = static_cast<T *>(const_cast<void *>(p.values));
+  const uint8_t *codes = p.codes, *scales = p.scales;
+  const long long rows = p.rows, units = p.units;
+  const int cols = p.cols, blocks = p.blocks, segments = static_cast<int>(p.segments);
   constexpr bool kDirect = ALIGNED && sizeof(T) == 2;
   __shared__ __align__(16) float sorted[kDirect ? 1 : kWarps][kDirect ? 4 : kSegment];
   hom::ptx::pdl_launch_dependents();
@@ -432,6 +451,19 @@ bool grid_fits(long long grid, const char *what) {
 
 bool is_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+Params params(const void *values, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t cols) {
+  Params p = {};
+  p.values = values;
+  p.codes = codes;
+  p.scales = scales;
+  p.rows = rows;
+  p.cols = static_cast<int>(cols);
+  p.blocks = static_cast<int>(blocks_of(cols));
+  p.segments = static_cast<uint32_t>((cols + kSegment - 1) / kSegment);
+  p.units = tile_rows_of(rows) * kRowStep * p.segments;
+  return p;
+}
+
 double traffic(int64_t rows, int64_t cols, size_t element) {
   return static_cast<double>(rows) * (static_cast<double>(cols) * element + 16.5 * blocks_of(cols));
 }
@@ -442,11 +474,10 @@ template <typename T>
 bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t cols,
               cudaStream_t stream) {
   const char *what = "4-bit quantisation launch";
-  const int64_t blocks = blocks_of(cols), tile_rows = tile_rows_of(rows);
-  const long long rows_ll = rows;
-  const int cols_i = static_cast<int>(cols), blocks_i = static_cast<int>(blocks);
+  const int64_t tile_rows = tile_rows_of(rows);
+  Params p = params(x, codes, scales, rows, cols);
   if (transposed) {
-    const int64_t tile_cols = tile_cols_of(blocks);
+    const int64_t tile_cols = tile_cols_of(p.blocks);
     if (!grid_fits(tile_rows, what)) return false;
     if (tile_cols > 65535) {
       set_error(HOM_ERR_UNSUPPORTED, "%s: a transposed matrix has at most 65535 x 128 values along K", what);
@@ -457,35 +488,26 @@ bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int6
     const bool two = kColumns == 2 && rows % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & 3u) == 0;
     return check_cuda(launch_pdl(two ? quantize_columns_kernel<T, kColumns> : quantize_columns_kernel<T, 1>,
                                  dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>(tile_cols)),
-                                 dim3(kTileRows / (two ? 2 : 1), kTileBlocks), 0, stream, 1, x, codes, scales, rows_ll,
-                                 cols_i, blocks_i),
+                                 dim3(kTileRows / (two ? 2 : 1), kTileBlocks), 0, stream, 1, p),
                       what);
   }
-  const int64_t segments = (cols + kSegment - 1) / kSegment;
-  const long long units = tile_rows * kRowStep * segments;
-  const long long grid = (units + kWarps - 1) / kWarps;
+  const long long grid = (p.units + kWarps - 1) / kWarps;
   if (!grid_fits(grid, what)) return false;
   auto kernel = cols % kLaneValues == 0 && is_aligned16(x) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
   LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
-  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, x, codes,
-                               scales, rows_ll, cols_i, blocks_i, static_cast<uint32_t>(segments), units),
-                    what);
+  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, p), what);
 }
 
 template <typename T>
 bool dequantize(const uint8_t *codes, const uint8_t *scales, T *out, int64_t rows, int64_t cols,
                 cudaStream_t stream) {
   const char *what = "4-bit dequantisation launch";
-  const int64_t blocks = blocks_of(cols), segments = (cols + kSegment - 1) / kSegment;
-  const long long units = tile_rows_of(rows) * kRowStep * segments;
-  const long long grid = (units + kWarps - 1) / kWarps;
+  const Params p = params(out, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols);
+  const long long grid = (p.units + kWarps - 1) / kWarps;
   if (!grid_fits(grid, what)) return false;
   auto kernel = cols % kLaneValues == 0 && is_aligned16(out) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
   LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
-  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, codes,
-                               scales, out, static_cast<long long>(rows), static_cast<int>(cols),
-                               static_cast<int>(blocks), static_cast<int>(segments), units),
-                    what);
+  return check_cuda(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(32 * kWarps), 0, stream, 1, p), what);
 }
 
 template bool quantize<__half>(const __half *, bool, uint8_t *, uint8_t *, int64_t, int64_t, cudaStream_t);

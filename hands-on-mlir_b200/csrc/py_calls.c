@@ -1,6 +1,6 @@
 /* Direct calls of the 4-bit and rotary entry points for the Python binding (module `hom_calls`).
  *
- * ctypes takes 1.3 to 2.5 us to convert the 7 to 15 arguments of such a call, on top of the 2 us
+ * ctypes takes 1.3 to 2.5 us to convert the 7 to 15 arguments of such a call, on top of the 1.7 us
  * that a launch costs the host, and the smallest of these operators run 1.5 to 2.5 us on the
  * device: a loop of them was bound by the conversion.  Here a memref argument is two attribute
  * reads.  Optional: built when the interpreter's headers are there (stable ABI), and the binding

@@ -29,7 +29,9 @@ struct Params {
   uint32_t chunks;              // a warp takes one token's heads
   int heads_per_chunk;          // [c * heads_per_chunk, ...)
   float magnitude, sign;
+  int fill[8];
 };
+static_assert(quick_to_launch<Params>, "see launch_pdl");
 
 template <typename T, int VEC>
 struct Vec;
@@ -217,7 +219,7 @@ __global__ void frequencies_kernel(double *out, int half, double base, int scali
 
 template <typename T, int VEC>
 bool launch(const Problem &pb, cudaStream_t stream) {
-  Params p;
+  Params p = {};
   p.x = pb.x.ptr;
   p.out = pb.out.ptr;
   p.x_b = pb.x.stride_b, p.x_s = pb.x.stride_s, p.x_h = pb.x.stride_h;
