@@ -135,7 +135,7 @@ PRODUCTS = [(1, 8, 32), (1, 4096, 1024), (2, 1, 32), (2, 333, 5000), (7, 33, 96)
             (127, 129, 256), (128, 128, 288), (129, 200, 544), (385, 1001, 808), (300, 1000, 800), (640, 512, 1056),
             (1100, 2304, 768), (2500, 1024, 520), (1001, 2001, 1060), (3900, 2400, 300), (4001, 2391, 600),
             (5, 72, 40000), (900, 1288, 2500), (100, 1001, 3000), (130, 1000, 2600), (128, 4000, 4200), (200, 777, 4100),
-            (20, 640, 1700)]
+            (20, 640, 1700), (4001, 2390, 600), (9500, 70, 300)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
