@@ -34,18 +34,8 @@ struct Params {
 static_assert(quick_to_launch<Params>, "see launch_pdl");
 
 template <typename T, int VEC>
-struct Vec;
-template <typename T>
-struct Vec<T, 1> {
-  T v[1];
-};
-template <>
-struct __align__(16) Vec<__half, 8> {
-  __half v[8];
-};
-template <>
-struct __align__(16) Vec<float, 4> {
-  float v[4];
+struct __align__(sizeof(T) * VEC) Vec {
+  T v[VEC];
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -261,13 +251,18 @@ bool launch(const Problem &pb, cudaStream_t stream) {
 
 template <typename T>
 bool run(const Problem &pb, cudaStream_t stream) {
-  constexpr int VEC = 16 / sizeof(T);
-  auto fits = [&](const View &v) {
-    return (reinterpret_cast<uintptr_t>(v.ptr) & 15u) == 0 && (pb.batch == 1 || v.stride_b % VEC == 0) &&
-           (pb.seq == 1 || v.stride_s % VEC == 0) && (pb.heads == 1 || v.stride_h % VEC == 0);
+  // The widest vectors, up to 16 bytes, that heads, their parts and all strides are whole ones of.
+  auto fits = [&](int64_t vec) {
+    auto view = [&](const View &v) {
+      return reinterpret_cast<uintptr_t>(v.ptr) % (vec * sizeof(T)) == 0 && (pb.batch == 1 || v.stride_b % vec == 0) &&
+             (pb.seq == 1 || v.stride_s % vec == 0) && (pb.heads == 1 || v.stride_h % vec == 0);
+    };
+    return pb.half % vec == 0 && (pb.dim - 2 * pb.half) % vec == 0 && view(pb.x) && view(pb.out);
   };
-  const bool vectors = pb.half % VEC == 0 && (pb.dim - 2 * pb.half) % VEC == 0 && fits(pb.x) && fits(pb.out);
-  return vectors ? launch<T, VEC>(pb, stream) : launch<T, 1>(pb, stream);
+  if constexpr (sizeof(T) == 2)
+    if (fits(8)) return launch<T, 8>(pb, stream);
+  if (fits(4)) return launch<T, 4>(pb, stream);
+  return fits(2) ? launch<T, 2>(pb, stream) : launch<T, 1>(pb, stream);
 }
 
 template bool run<__half>(const Problem &, cudaStream_t);
