@@ -74,15 +74,16 @@ __device__ __forceinline__ void apply_turns(Vec<T, VEC> &first, Vec<T, VEC> &sec
 
 // One warp per token, or per token and group of heads where there are too few tokens to fill the
 // chip.  The warp forms the token's sines and cosines once, in shared memory, and walks over its
-// heads; a task is VEC pairs of a head, two 16-byte vectors, or two vectors of its other dimensions,
-// which are copied.  The first tasks' loads are under way while the sines are formed.
+// heads; a task is VEC pairs of a head, two vectors of up to 16 bytes, or two vectors of its other
+// dimensions, which are copied.  The first tasks' loads are under way while the sines are formed.
 //
 // FIXED: the tasks of a head are a power of two up to 32 and all turn pairs, so that a lane works on
 // the same pairs of every head and keeps their sines and cosines in registers (64 x 512 tokens of 32
 // heads: 65 us without).
 //
-// Bound by memory: each element is read and written once, 64 x 512 x 32 heads x 64 fp16 values in
-// 41.1 us, 6.5 TB/s.  Four CTAs on an SM with two tasks a lane in flight; three CTAs with four took
+// Bound by memory where a token has many heads: each element is read and written once, 64 x 512 x 32
+// heads x 64 fp16 values in 41.1 us, 6.5 TB/s; otherwise by what a token costs (32 x 512 x 12 heads x
+// 128 32.5 us, 3.1 TB/s).  Four CTAs on an SM with two tasks a lane in flight; three CTAs with four took
 // 47 us, six with one 45.
 template <typename T, int VEC, bool INTERLEAVED, bool FIXED>
 __global__ void __launch_bounds__(32 * kWarps, 4) rotary_kernel(const Params p) {
