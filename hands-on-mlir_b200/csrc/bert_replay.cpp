@@ -68,7 +68,8 @@ struct Program {
   Tensor x, type_rows, qkv, ctx, ffn, cu;  // activations (hoisted allocations)
   Tensor stats[2];  // fused_layernorm == 2: fp32 row partial sums of the raw hidden states (ping-pong)
   Tensor ids_dev, mask_dev, types_dev;     // staging for the host entry point
-  cudaStream_t own_stream = nullptr;
+  cudaStream_t own_stream = nullptr;       // to capture on for a caller on the legacy default stream
+  cudaEvent_t hand_over = nullptr;         // between that stream and the caller's
   cudaGraphExec_t graph_exec = nullptr;
   // pipelined host entry point: two device result slots, a copy stream and hand-off events
   Tensor result_slot[2];
@@ -288,6 +289,16 @@ int issue_forward(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void
   return status();
 }
 
+// What is issued to `after` from now on waits for what was issued to `before` so far.
+bool order_streams(Program &p, cudaStream_t before, cudaStream_t after) {
+  if (!p.hand_over && cudaEventCreateWithFlags(&p.hand_over, cudaEventDisableTiming) != cudaSuccess) {
+    p.hand_over = nullptr;
+    return false;
+  }
+  return cudaEventRecord(p.hand_over, before) == cudaSuccess &&
+         cudaStreamWaitEvent(after, p.hand_over, 0) == cudaSuccess;
+}
+
 int forward_impl(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void *mask,
                  int64_t rankTypes, void *types, int use_graph) {
   if (!ready(p)) return HOM_ERR_INVALID;
@@ -317,8 +328,18 @@ int forward_impl(Program &p, int64_t rankIds, void *ids, int64_t rankMask, void 
     }
     if (p.warm_stream != stream || !p.warm_stream_valid) {
       // Per-stream scratch of the library (the split-K workspace) is allocated on a stream's
-      // first use, which must not happen during capture: run once eagerly on this stream.
-      const int wrc = issue_forward(p, rankIds, ids, rankMask, mask, rankTypes, types);
+      // first use, which must not happen during capture: run once eagerly on this stream.  Where it
+      // is the program's own, that run works on the same buffers as what the caller's stream did
+      // before and does next, and nothing but events orders the two.  (A forward beside another one
+      // does not only compute nonsense: thrustCuSeqLenI64 leaves row lengths where the prefix sums
+      // belong for a moment, and an attention CTA whose warps read two different lengths waits until
+      // its limit, so that the GEMM behind it may report an expired wait first.)
+      const bool own = stream != user_stream;
+      int wrc = own && !order_streams(p, user_stream, stream) ? HOM_ERR_CUDA : 0;
+      if (wrc == 0) {
+        wrc = issue_forward(p, rankIds, ids, rankMask, mask, rankTypes, types);
+        if (own && !order_streams(p, stream, user_stream) && wrc == 0) wrc = HOM_ERR_CUDA;
+      }
       if (wrc != 0) {
         homSetStream(user_stream);
         return wrc;
@@ -402,6 +423,7 @@ void homBertDestroy(void *program) {
   for (int i = 0; i < 2; ++i)
     if (p->host_graph[i]) cudaGraphExecDestroy(p->host_graph[i]);
   if (p->own_stream) cudaStreamDestroy(p->own_stream);
+  if (p->hand_over) cudaEventDestroy(p->hand_over);
   if (p->copy_stream) {
     cudaStreamSynchronize(p->copy_stream);
     cudaStreamDestroy(p->copy_stream);
