@@ -457,6 +457,7 @@ int homBertSetWeight(void *program, int32_t index, int64_t rank, void *descripto
   if (!p || index < 0 || index >= static_cast<int32_t>(p->weights.size()) || !descriptor ||
       rank != 3)
     return HOM_ERR_INVALID;
+  forget_graphs(*p);  // the captured calls name the buffers bound so far
   release(p->weights[index], true);
   p->coded_stale = true;
   // Copy the descriptor record so the caller's may go away; the buffer stays the caller's.
@@ -477,16 +478,13 @@ int homBertSetWeight(void *program, int32_t index, int64_t rank, void *descripto
     homDeclareWeights(first, 2 * n);
     p->weights[index].declared = first;
   }
-  if (p->graph_exec) {
-    cudaGraphExecDestroy(p->graph_exec);
-    p->graph_exec = nullptr;
-  }
   return 0;
 }
 
 int homBertLoadConstants(void *program, int32_t first_idx) {
   auto *p = static_cast<Program *>(program);
   if (!p) return HOM_ERR_INVALID;
+  forget_graphs(*p);
   p->coded_stale = true;
   for (size_t i = 0; i < p->weights.size(); ++i) {
     release(p->weights[i], true);

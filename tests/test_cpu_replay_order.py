@@ -25,3 +25,9 @@ def ordering(tmp_path_factory):
 def test_every_call_comes_after_the_one_before(ordering, scenario):
     run = subprocess.run([str(ordering), scenario], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
+
+
+@pytest.mark.parametrize("scenario", ["new_weights", "new_constants"])
+def test_no_graph_outlives_its_weights(ordering, scenario):
+    run = subprocess.run([str(ordering), scenario], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stdout + run.stderr
