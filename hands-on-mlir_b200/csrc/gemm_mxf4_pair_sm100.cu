@@ -294,11 +294,13 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         else tma_load_3d_pair(dst + kCodeBytes, &tmSB, bar, 0, step * kStepTiles, n0 / kTileRows);
       };
       // The first round of stages is armed, and a declared B requested, before the previous kernel
-      // has finished.
+      // has finished; the ring's stages are free the first time round, so that no wait with a limit
+      // comes before the one for that kernel.
       int early = first < last ? min(kStages, p.steps) : 0, a_early = early;
       if (arms)
         for (int i = 0; i < early; ++i) mbar_arrive_expect_tx(armed_bar + 8 * i, armed_bytes);
-      if (warp != 2 || !p.b_early) pdl_wait();
+      bool waits = warp == 2 && p.b_early;  // still has the previous kernel to wait for
+      if (!waits) pdl_wait();
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
       for (int tile = first; tile < last && ok; tile += stride) {
@@ -328,6 +330,10 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           if (++slot == kStages) {
             slot = 0;
             ph ^= 1u;
+            if (waits) {
+              pdl_wait();
+              waits = false;
+            }
           }
         }
         if (new_a) a_ph ^= 1u;
@@ -346,6 +352,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
       int it = 0, n_block = first % p.n_blocks;  // (where A is resident)
+      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       for (int tile = first; tile < last && ok; tile += stride, ++it) {
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + (acc ? kSecondAcc : 0);

@@ -202,8 +202,10 @@ gemm_f16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       uint32_t dst = smem_base + kABytes, slot = 0, ph = 0;
       bool ok = true;
       const bool b_grouped = p.b_grouped != 0;
-      // A declared constant is requested without waiting for the previous kernel (gemm_sm100.cu).
-      if (!p.b_early) pdl_wait();
+      // A declared constant is requested without waiting for the previous kernel, one ring of it
+      // (gemm_sm100.cu).
+      bool early = p.b_early != 0;
+      if (!early) pdl_wait();
       for (int unit = pair; unit < p.num_units && ok; unit += num_pairs) {
         const int tile = unit / p.split_k, part = unit % p.split_k;
         const int nb0 = (tile % p.n_blocks) * BN2 + static_cast<int>(rank) * HALF;
@@ -226,6 +228,10 @@ gemm_f16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             dst = smem_base + kABytes;
             slot = 0;
             ph ^= 1u;
+            if (early) {
+              pdl_wait();
+              early = false;
+            }
           }
         }
       }
@@ -243,6 +249,7 @@ gemm_f16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       uint32_t bar = full_bar(0), ph = 0;
       bool ok = true;
       int it = 0;
+      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       HOM_DIAG(long long t_full = 0, t_acc = 0; const long long t_begin = clock64();)
       for (int unit = pair; unit < p.num_units && ok; unit += num_pairs, ++it) {
         const int part = unit % p.split_k;

@@ -211,8 +211,10 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       // A declared constant (weights, which no kernel of the stream writes) is requested without
       // waiting for the previous kernel: the first ring of B tiles then arrives while that one
       // finishes.  A B of unknown origin only after.  (Its bytes may land before the A warp has
-      // armed the barrier: the phase cannot complete without that arrival.)
-      if (!p.b_early) pdl_wait();
+      // armed the barrier: the phase cannot complete without that arrival.)  The ring's stages are
+      // free the first time round, so no wait with a limit comes before the one for that kernel.
+      bool early = p.b_early != 0;
+      if (!early) pdl_wait();
       for (int unit = blockIdx.x; unit < p.num_units && ok; unit += gridDim.x) {
         const int tile = unit / p.split_k, part = unit % p.split_k;
         const int n0 = (tile % p.n_blocks) * BN;
@@ -234,6 +236,10 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             dst = smem_base + kABytes;
             bar = full_bar(0);
             ph ^= 1u;
+            if (early) {
+              pdl_wait();
+              early = false;
+            }
           }
         }
       }
@@ -259,6 +265,7 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       uint32_t bar = full_bar(0), ph = 0;
       bool ok = true;
       int it = 0;
+      pdl_wait();  // the limits of the waits below are for this kernel's work, not for the previous one's
       HOM_DIAG(long long t_full = 0, t_acc = 0; const long long t_begin = clock64();)
       for (int unit = blockIdx.x; unit < p.num_units && ok; unit += gridDim.x, ++it) {
         const int part = unit % p.split_k;
