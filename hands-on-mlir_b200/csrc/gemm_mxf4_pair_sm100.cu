@@ -434,6 +434,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const int m_stride = stride / p.n_blocks, n_stride = stride - m_stride * p.n_blocks;
     uint32_t next_row = row && first < last ? load_row(n_block) : 0u;
     int it = 0;
+    bool ok = true;
     for (int tile = first; tile < last; tile += stride, ++it) {
       const int acc = it & 1;
       const int row0 = m_block * BM + static_cast<int>(rank) * kHalf + quarter * 32;
@@ -458,7 +459,7 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         mbar_arrive_expect_tx(c_bar(drain), gemm::kEpilogueTileBytes);
         tma_load_2d(stage_smem, &tmC, c_bar(drain), c0, row0);
       }
-      bool ok = mbar_wait(acc_full_bar(acc), (it >> 1) & 1, abort_flag, p.status, kDevWaitTimeoutEpilogue);
+      ok = mbar_wait(acc_full_bar(acc), (it >> 1) & 1, abort_flag, p.status, kDevWaitTimeoutEpilogue);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
@@ -523,7 +524,14 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         bulk_commit_group();
       }
     }
-    if (lane == 0) bulk_wait_group_read_0();
+    if (lane == 0) {
+      if (full && !ragged && !ok) {  // C's block may still be on its way into the staging tile
+        const long long t0 = clock64();
+        while (!mbar_try_wait(c_bar(drain), it & 1) && clock64() - t0 < 400000000LL) {
+        }
+      }
+      bulk_wait_group_read_0();
+    }
     __syncwarp();
   }
 
