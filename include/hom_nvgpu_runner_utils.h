@@ -185,8 +185,9 @@ HOM_EXPORT int homSynchronize(void);
  * (model weights).  Kernels of this library are launched so that one may start while the previous
  * kernel of the stream is still finishing; a GEMM requests its first tiles of a DECLARED B before
  * that previous kernel is known to be complete, and those of any other B only afterwards, so a B
- * that an earlier call on the stream produced is always read after it was written.  Buffers
- * returned by allocConstantNVGPU* are declared by the library; callers that bring their own
+ * that an earlier call on the stream produced is always read after it was written.  What writes a
+ * buffer must therefore be complete (homSynchronize) before the first call that reads it as
+ * declared.  Buffers returned by allocConstantNVGPU* are declared by the library; callers that bring their own
  * weight buffers may declare them to get the earlier prefetch.  homForgetWeights() withdraws a
  * declaration (call it before the buffer is freed or reused).  What the library derives from a
  * declared weight and keeps (a re-pitched copy for N % 8 != 0; column sums for
@@ -302,7 +303,9 @@ HOM_EXPORT void homLayernormGemmF16NoAlloc(int64_t rankA, void *dstA, int64_t ra
  * over it are rounded to the nearest code, ties to even, magnitudes above 6 to 6.  A block that
  * holds a NaN or an infinity becomes NaN as a whole.  X [.., rows, K] (any element alignment), or
  * [K, rows] / [1, K, rows] with `transposed` (a weight stored [1,K,N]): the blocks run along K
- * either way.  All of Q and S is written.
+ * either way.  All of Q and S is written, and a declaration (homDeclareWeights) that holds any of
+ * it is withdrawn: products after this call read it only after it was written, and fetch it early
+ * again once it is declared anew.
  * homDequantizeMxF4*: Out [.., rows, K] = the values; exact in fp32, in fp16 wherever the values
  * came from fp16.
  * No counterpart in the reference, whose path is fp16 throughout. */
@@ -319,7 +322,8 @@ HOM_EXPORT void homDequantizeMxF4F32(int64_t rankQ, void *dstQ, int64_t rankS, v
  * [1, N, K] with equal numbers of blocks: the 4-bit counterpart of nvteGemmF16 with its epilogue
  * (fp32 accumulation; fp16 C and D; C [.., M, N], which may be D, or one row of N; unused when
  * beta == 0; `activation` 1 = erf GELU).  D (and C) 16-byte aligned when N % 8 == 0.  Q and S of
- * the weight may be declared (homDeclareWeights, one declaration each) to be fetched early. */
+ * the weight may be declared (homDeclareWeights, one declaration each) to be fetched early: after
+ * the stream that quantised them was waited for. */
 HOM_EXPORT void homGemmMxF4F16(int64_t rankA, void *dstA, int64_t rankSA, void *dstSA, int64_t rankB,
                                void *dstB, int64_t rankSB, void *dstSB, int64_t rankC, void *dstC,
                                int64_t rankD, void *dstD, int64_t activation, float alpha, float beta);

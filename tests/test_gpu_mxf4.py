@@ -383,3 +383,40 @@ def test_two_threads_on_two_streams(hom, pkg, cuda):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("m", [1, 2, 200, 3000])
+def test_declared_weights_and_their_rewriting(hom, pkg, cuda, m):
+    """Every form of the product with a declared weight, and right behind a call that quantises another weight into the
+    declared buffers, with nothing that waits in between."""
+    import torch
+
+    n, k = 2048, 1600
+    rng = np.random.default_rng(m)
+    x = to_dev(rng.standard_normal((m, k)).astype(np.float16), cuda)
+    ws = [to_dev(rng.standard_normal((n, k)).astype(np.float32), cuda) for _ in range(2)]
+    (aq, _), (as_, _) = _buffers(pkg, cuda, m, k)
+    (bq, b_all), (bs, s_all) = _buffers(pkg, cuda, n, k)
+    d = [torch.empty((m, n), dtype=torch.float16, device=cuda) for _ in range(6)]
+    for w, out in zip(ws, d):
+        hom.homQuantizeMxF4F32(w, bq, bs)
+        hom.homQuantizeMxF4F16(x, aq, as_)
+        hom.homGemmMxF4F16(aq, as_, bq, bs, None, out)
+    hom.synchronize()
+    assert not torch.equal(d[0], d[1])
+    try:
+        for _ in range(3):
+            # (one declaration around the codes, more than they take)
+            hom.declare_weights(b_all)
+            hom.declare_weights(bs)
+            hom.homQuantizeMxF4F16(x, aq, as_)
+            hom.homGemmMxF4F16(aq, as_, bq, bs, None, d[2])
+            for w, out in zip(ws, d[3:5]):
+                hom.homQuantizeMxF4F32(w, bq, bs)
+                hom.homQuantizeMxF4F16(x, aq, as_)
+                hom.homGemmMxF4F16(aq, as_, bq, bs, None, out)
+            hom.synchronize()
+            assert torch.equal(d[2], d[1]) and torch.equal(d[3], d[0]) and torch.equal(d[4], d[1])
+    finally:
+        hom.forget_weights(b_all)
+        hom.forget_weights(bs)
