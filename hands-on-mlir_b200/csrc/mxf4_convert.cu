@@ -306,7 +306,13 @@ quantize_rows_kernel(const Params p) {
 // CTA makes one scale tile, whose bytes it gathers in shared memory.  Two columns for fp16 (rows even,
 // x on 4 bytes): a [4096, 4096] weight takes 14.1 us (3.0 TB/s: pieces of 256 bytes out of rows of
 // 8 KB), with 2-byte loads 27.7.
-template <typename T, int COLUMNS>
+//
+// The scale tiles along K are the grid's second dimension, which ends at 65535.  LONG: the third takes
+// what is beyond.  (An instantiation of its own: the loads are scheduled so finely that the additional
+// index took [4096, 4096] from 13.4 to 15.6 us, and one dimension with a division to 15.0.)
+constexpr int64_t kMaxGridY = 65535;
+
+template <typename T, int COLUMNS, bool LONG>
 __global__ void __launch_bounds__(kTileRows * kTileBlocks / COLUMNS)
 quantize_columns_kernel(const Params p) {
   const T *x = static_cast<const T *>(p.values);
@@ -320,7 +326,10 @@ quantize_columns_kernel(const Params p) {
   };
   const int r0 = static_cast<int>(threadIdx.x) * COLUMNS, b = threadIdx.y;
   const long long row0 = static_cast<long long>(blockIdx.x) * kTileRows + r0;
-  const int block = static_cast<int>(blockIdx.y) * kTileBlocks + b;
+  const uint32_t tile_cols = LONG ? (blocks + kTileBlocks - 1) / kTileBlocks : gridDim.y;
+  const uint32_t tile_col = LONG ? blockIdx.z * gridDim.y + blockIdx.y : blockIdx.y;
+  if (LONG && tile_col >= tile_cols) return;
+  const int block = static_cast<int>(tile_col) * kTileBlocks + b;
   const T *from = x + static_cast<long long>(block) * kBlock * rows + row0;
   Few v[kBlock];
 #pragma unroll
@@ -366,7 +375,7 @@ quantize_columns_kernel(const Params p) {
   __syncthreads();
   const int t = static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x);
   if (t < kTileBytes / 16)
-    reinterpret_cast<uint4 *>(p.scales + (static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y) * kTileBytes)[t] =
+    reinterpret_cast<uint4 *>(p.scales + (static_cast<long long>(blockIdx.x) * tile_cols + tile_col) * kTileBytes)[t] =
         reinterpret_cast<const uint4 *>(tile_bytes)[t];
 }
 
@@ -479,15 +488,16 @@ bool quantize(const T *x, bool transposed, uint8_t *codes, uint8_t *scales, int6
   if (transposed) {
     const int64_t tile_cols = tile_cols_of(p.blocks);
     if (!grid_fits(tile_rows, what)) return false;
-    if (tile_cols > 65535) {
-      set_error(HOM_ERR_UNSUPPORTED, "%s: a transposed matrix has at most 65535 x 128 values along K", what);
-      return false;
-    }
+    const int64_t slices = (tile_cols + kMaxGridY - 1) / kMaxGridY;
     LaunchScope scope(kOpConvert, 0.0, traffic(rows, cols, sizeof(T)));
     constexpr int kColumns = sizeof(T) == 2 ? 2 : 1;
-    const bool two = kColumns == 2 && rows % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & 3u) == 0;
-    return check_cuda(launch_pdl(two ? quantize_columns_kernel<T, kColumns> : quantize_columns_kernel<T, 1>,
-                                 dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>(tile_cols)),
+    const bool two = kColumns == 2 && slices == 1 && rows % 2 == 0 && (reinterpret_cast<uintptr_t>(x) & 3u) == 0;
+    auto kernel = two          ? quantize_columns_kernel<T, kColumns, false>
+                  : slices > 1 ? quantize_columns_kernel<T, 1, true>
+                               : quantize_columns_kernel<T, 1, false>;
+    return check_cuda(launch_pdl(kernel,
+                                 dim3(static_cast<unsigned>(tile_rows), static_cast<unsigned>((tile_cols + slices - 1) / slices),
+                                      static_cast<unsigned>(slices)),
                                  dim3(kTileRows / (two ? 2 : 1), kTileBlocks), 0, stream, 1, p),
                       what);
   }

@@ -420,3 +420,22 @@ def test_declared_weights_and_their_rewriting(hom, pkg, cuda, m):
     finally:
         hom.forget_weights(b_all)
         hom.forget_weights(bs)
+
+
+@pytest.mark.parametrize("rows,dtype", [(2, np.float16), (1, np.float32)])
+def test_quantize_transposed_with_a_long_k(hom, pkg, cuda, rows, dtype):
+    """More than 2^16 scale tiles along K."""
+    cols = 128 * 65536 + 33
+    x = np.random.default_rng(rows).standard_normal((cols, rows)).astype(dtype)
+    (q, q_all), (s, s_all) = buffers = _buffers(pkg, cuda, rows, cols)
+    (hom.homQuantizeMxF4F16 if dtype == np.float16 else hom.homQuantizeMxF4F32)(to_dev(x, cuda), q, s, True)
+    q, s = q.cpu().numpy(), s.cpu().numpy()
+    _assert_guards(buffers)
+    for first in (0, 128 * 32768, 128 * 65535, 128 * 65536):  # blocks are independent of one another
+        part = x[first:first + 128].T
+        codes, scales = ref.quantize(part)
+        assert np.array_equal(q[:, first // 2:first // 2 + codes.shape[1]], codes)
+        assert np.array_equal(s[:, first // 128:first // 128 + 1], ref.tile_scales(scales))
+    rq, rs = ([v for v, _ in _buffers(pkg, cuda, rows, cols)])
+    (hom.homQuantizeMxF4F16 if dtype == np.float16 else hom.homQuantizeMxF4F32)(to_dev(x.T, cuda), rq, rs)
+    assert np.array_equal(rq.cpu().numpy(), q) and np.array_equal(rs.cpu().numpy(), s)
