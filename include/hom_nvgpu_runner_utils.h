@@ -335,9 +335,11 @@ HOM_EXPORT void homGemmMxF4F16(int64_t rankA, void *dstA, int64_t rankSA, void *
  * `backward` applies the transpose, which takes the gradient of Out to that of X.  Dimensions
  * beyond 2F are copied.  X, Out [bs, seq, heads, d] with any non-negative strides and a contiguous
  * last dimension - the query and key heads of a packed [bs, seq, 3*heads*d] are the view
- * [bs, seq, 2*heads, d] of it -; Out may be X, otherwise they must not overlap.  Positions int64
- * [bs, seq] or [1, seq], absent (rank 0 / null): 0 .. seq - 1; bs * seq and heads * d below 2^31.
- * Frequencies fp64 [F], F <= 512;
+ * [bs, seq, 2*heads, d] of it -.  Out may be X; otherwise its addresses, from the first to the last
+ * element, must not meet those of X (which those of two groups of heads of one packed buffer do),
+ * nor in any case those of Positions and Frequencies; and its dimensions, in the order of their
+ * strides, must each lie within one step of the next.  Positions int64 [bs, seq] or [1, seq], absent
+ * (rank 0 / null): 0 .. seq - 1; bs * seq and heads * d below 2^31.  Frequencies fp64 [F], F <= 512;
  * angles are formed in 64 bits, so that far positions keep their fractions of a turn.  The
  * rotation is fp32, rounded once.
  * No counterpart in the reference, whose model adds a position table. */

@@ -122,6 +122,19 @@ def test_rotary_refusals(pkg, hom, nothing_launched, name, element):
     _refused(pkg, 2, "2^30", call, pkg.MemRef(16, ((1 << 30) + 1, 1, 1, 8)), None, f, pkg.MemRef(16, ((1 << 30) + 1, 1, 1, 8)))
 
 
+def test_rotary_overlap_is_a_matter_of_address_ranges(pkg, hom, nothing_launched):
+    """Two groups of heads of one packed buffer share no element and are refused all the same, as are dimensions of Out
+    that interleave."""
+    packed = _host(pkg, (2, 3, 12, 8), 2)
+    query, key = (pkg.MemRef(packed.data_ptr + 2 * 8 * first, (2, 3, 4, 8), (288, 96, 8, 1)) for first in (0, 4))
+    f = _host(pkg, (4,), 8)
+    _refused(pkg, 1, "overlaps", hom.homRotaryF16, query, None, f, key)
+    _refused(pkg, 1, "overlaps", hom.homRotaryF16, key, None, f, query)
+    out = _host(pkg, (8, 8), 2)  # pieces of eight at 0, 2, 4 and 3, 5, 7
+    _refused(pkg, 1, "share memory", hom.homRotaryF16, _host(pkg, (2, 3, 1, 8), 2), None, f,
+             pkg.MemRef(out.data_ptr, (2, 3, 1, 8), (24, 16, 8, 1)))
+
+
 def test_frequency_refusals(pkg, hom, nothing_launched):
     f = _host(pkg, (4,), 8)
     call = hom.homRotaryFrequencies
