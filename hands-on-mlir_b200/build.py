@@ -115,7 +115,8 @@ def _build_calls(lib_dir: Path, runner_lib: Path, force: bool, verbose: bool) ->
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"building {out.name} failed:\n{proc.stdout}\n{proc.stderr}")
+        out.unlink(missing_ok=True)  # (one of an earlier build may be out of date)
+        print(f"hom_calls: cannot be built, the binding uses ctypes:\n{proc.stdout}\n{proc.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False, diagnostics: bool = False) -> dict[str, Path]:

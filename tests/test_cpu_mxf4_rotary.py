@@ -194,3 +194,26 @@ def test_direct_calls_and_ctypes_agree(pkg, hom, nothing_launched):
         with pytest.raises(Exception) as e:
             h.homGemmMxF4F16(*a, *b, None, _host(pkg, (6, 16), 2), alpha="one")
         assert not isinstance(e.value, pkg.HomError)
+
+
+def test_a_failed_build_of_the_direct_calls_is_no_failed_build(tmp_path, monkeypatch, capsys):
+    """The module is optional: what cannot be compiled is left out, an outdated one of an earlier build included."""
+    import importlib.util
+    import stat
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("hom_build_calls", Path(__file__).parents[1] / "hands-on-mlir_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    compiler = tmp_path / "gcc"
+    compiler.write_text("#!/bin/sh\necho no such option >&2\nexit 1\n")
+    compiler.chmod(compiler.stat().st_mode | stat.S_IXUSR)
+    monkeypatch.setenv("PATH", str(tmp_path))
+    headers = tmp_path / "include"
+    headers.mkdir()
+    (headers / "Python.h").write_text("")
+    monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(headers)})
+    old = tmp_path / build.CALLS_MODULE
+    old.write_bytes(b"")
+    build._build_calls(tmp_path, tmp_path / build.RUNNER_LIB.name, True, False)
+    assert not old.exists() and "no such option" in capsys.readouterr().out
