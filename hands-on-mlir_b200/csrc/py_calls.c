@@ -13,9 +13,12 @@
 
 #include "hom_nvgpu_runner_utils.h"
 
-static PyTypeObject *memref_type;    /* the binding's MemRef */
-static PyObject *to_memref;          /* makes one of a tensor */
-static PyObject *s_rank, *s_address; /* attribute names */
+/* One for each time the module is loaded: every copy of the package has a MemRef of its own. */
+typedef struct {
+  PyTypeObject *memref_type;    /* the binding's MemRef */
+  PyObject *to_memref;          /* makes one of a tensor */
+  PyObject *s_rank, *s_address; /* attribute names */
+} State;
 
 enum { kMaxMemrefs = 6 };
 typedef struct {
@@ -29,18 +32,22 @@ static void release(Memrefs *m) {
   for (int i = 0; i < m->count; ++i) Py_XDECREF(m->made[i]);
 }
 
-static int take(Memrefs *m, PyObject *x) {
+static int take(const State *state, Memrefs *m, PyObject *x) {
   const int i = m->count++;
   m->rank[i] = 0;
   m->descriptor[i] = NULL;
   m->made[i] = NULL;
   if (x == Py_None) return 1;
-  if (Py_TYPE(x) != memref_type) {
-    x = m->made[i] = PyObject_CallFunctionObjArgs(to_memref, x, NULL);
+  if (!state->memref_type) {
+    PyErr_SetString(PyExc_RuntimeError, "hom_calls: not bound");
+    return 0;
+  }
+  if (Py_TYPE(x) != state->memref_type && !PyType_IsSubtype(Py_TYPE(x), state->memref_type)) {
+    x = m->made[i] = PyObject_CallFunctionObjArgs(state->to_memref, x, NULL);
     if (!x) return 0;
   }
-  PyObject *rank = PyObject_GetAttr(x, s_rank);
-  PyObject *address = rank ? PyObject_GetAttr(x, s_address) : NULL;
+  PyObject *rank = PyObject_GetAttr(x, state->s_rank);
+  PyObject *address = rank ? PyObject_GetAttr(x, state->s_address) : NULL;
   if (address) {
     m->rank[i] = PyLong_AsLongLong(rank);
     m->descriptor[i] = PyLong_AsVoidPtr(address);
@@ -63,11 +70,12 @@ static PyObject *outcome(void) {
 }
 
 typedef void (*Quantize)(int64_t, void *, bool, int64_t, void *, int64_t, void *);
-static PyObject *quantize(Quantize call, const char *name, PyObject *const *args, Py_ssize_t n) {
+static PyObject *quantize(PyObject *self, Quantize call, const char *name, PyObject *const *args, Py_ssize_t n) {
+  const State *state = PyModule_GetState(self);
   Memrefs m = {.count = 0};
   if (!arguments(name, n, 4)) return NULL;
   const int transposed = PyObject_IsTrue(args[3]);
-  if (transposed < 0 || !take(&m, args[0]) || !take(&m, args[1]) || !take(&m, args[2])) {
+  if (transposed < 0 || !take(state, &m, args[0]) || !take(state, &m, args[1]) || !take(state, &m, args[2])) {
     release(&m);
     return NULL;
   }
@@ -79,10 +87,11 @@ static PyObject *quantize(Quantize call, const char *name, PyObject *const *args
 }
 
 typedef void (*Dequantize)(int64_t, void *, int64_t, void *, int64_t, void *);
-static PyObject *dequantize(Dequantize call, const char *name, PyObject *const *args, Py_ssize_t n) {
+static PyObject *dequantize(PyObject *self, Dequantize call, const char *name, PyObject *const *args, Py_ssize_t n) {
+  const State *state = PyModule_GetState(self);
   Memrefs m = {.count = 0};
   if (!arguments(name, n, 3)) return NULL;
-  if (!take(&m, args[0]) || !take(&m, args[1]) || !take(&m, args[2])) {
+  if (!take(state, &m, args[0]) || !take(state, &m, args[1]) || !take(state, &m, args[2])) {
     release(&m);
     return NULL;
   }
@@ -94,13 +103,13 @@ static PyObject *dequantize(Dequantize call, const char *name, PyObject *const *
 }
 
 static PyObject *product(PyObject *self, PyObject *const *args, Py_ssize_t n) {
-  (void)self;
+  const State *state = PyModule_GetState(self);
   Memrefs m = {.count = 0};
   if (!arguments("homGemmMxF4F16", n, 9)) return NULL;
   const long long activation = PyLong_AsLongLong(args[6]);
   const double alpha = PyFloat_AsDouble(args[7]), beta = PyFloat_AsDouble(args[8]);
   int ok = !PyErr_Occurred();
-  for (int i = 0; ok && i < 6; ++i) ok = take(&m, args[i]);
+  for (int i = 0; ok && i < 6; ++i) ok = take(state, &m, args[i]);
   if (!ok) {
     release(&m);
     return NULL;
@@ -115,13 +124,14 @@ static PyObject *product(PyObject *self, PyObject *const *args, Py_ssize_t n) {
 }
 
 typedef void (*Rotary)(int64_t, void *, int64_t, void *, int64_t, void *, int64_t, void *, bool, bool, float);
-static PyObject *rotary(Rotary call, const char *name, PyObject *const *args, Py_ssize_t n) {
+static PyObject *rotary(PyObject *self, Rotary call, const char *name, PyObject *const *args, Py_ssize_t n) {
+  const State *state = PyModule_GetState(self);
   Memrefs m = {.count = 0};
   if (!arguments(name, n, 7)) return NULL;
   const int interleaved = PyObject_IsTrue(args[4]), backward = PyObject_IsTrue(args[5]);
   const double magnitude = PyFloat_AsDouble(args[6]);
   int ok = interleaved >= 0 && backward >= 0 && !PyErr_Occurred();
-  for (int i = 0; ok && i < 4; ++i) ok = take(&m, args[i]);
+  for (int i = 0; ok && i < 4; ++i) ok = take(state, &m, args[i]);
   if (!ok) {
     release(&m);
     return NULL;
@@ -136,8 +146,7 @@ static PyObject *rotary(Rotary call, const char *name, PyObject *const *args, Py
 
 #define FORWARD(NAME, THROUGH)                                                          \
   static PyObject *NAME##_(PyObject *self, PyObject *const *args, Py_ssize_t n) {       \
-    (void)self;                                                                         \
-    return THROUGH(NAME, #NAME, args, n);                                               \
+    return THROUGH(self, NAME, #NAME, args, n);                                         \
   }
 FORWARD(homQuantizeMxF4F16, quantize)
 FORWARD(homQuantizeMxF4F32, quantize)
@@ -149,14 +158,19 @@ FORWARD(homRotaryF32, rotary)
 /* bind(MemRef, MemRef.of): the descriptor type, with the attributes `rank` and `address`, and what
  * makes one of anything else. */
 static PyObject *bind(PyObject *self, PyObject *const *args, Py_ssize_t n) {
-  (void)self;
+  State *state = PyModule_GetState(self);
   if (!arguments("bind", n, 2)) return NULL;
+  if (!PyType_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind takes a class and what makes one of its objects");
+    return NULL;
+  }
+  PyObject *type = (PyObject *)state->memref_type, *make = state->to_memref;
   Py_INCREF(args[0]);
   Py_INCREF(args[1]);
-  Py_XDECREF((PyObject *)memref_type);
-  Py_XDECREF(to_memref);
-  memref_type = (PyTypeObject *)args[0];
-  to_memref = args[1];
+  state->memref_type = (PyTypeObject *)args[0];
+  state->to_memref = args[1];
+  Py_XDECREF(type);
+  Py_XDECREF(make);
   Py_RETURN_NONE;
 }
 
@@ -172,10 +186,34 @@ static PyMethodDef methods[] = {
     METHOD("homRotaryF32", homRotaryF32_),
     {NULL, NULL, 0, NULL},
 };
-static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "hom_calls", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
-PyMODINIT_FUNC PyInit_hom_calls(void) {
-  s_rank = PyUnicode_InternFromString("rank");
-  s_address = PyUnicode_InternFromString("address");
-  return s_rank && s_address ? PyModule_Create(&module) : NULL;
+static int execute(PyObject *self) {
+  State *state = PyModule_GetState(self);
+  state->s_rank = PyUnicode_InternFromString("rank");
+  state->s_address = PyUnicode_InternFromString("address");
+  return state->s_rank && state->s_address ? 0 : -1;
 }
+
+static int traverse(PyObject *self, visitproc visit, void *arg) {
+  State *state = PyModule_GetState(self);
+  Py_VISIT(state->memref_type);
+  Py_VISIT(state->to_memref);
+  return 0;
+}
+
+static int clear(PyObject *self) {
+  State *state = PyModule_GetState(self);
+  Py_CLEAR(state->memref_type);
+  Py_CLEAR(state->to_memref);
+  Py_CLEAR(state->s_rank);
+  Py_CLEAR(state->s_address);
+  return 0;
+}
+
+static void release_state(void *self) { clear(self); }
+
+static PyModuleDef_Slot slots[] = {{Py_mod_exec, execute}, {0, NULL}};
+static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "hom_calls", NULL, sizeof(State), methods, slots, traverse, clear,
+                                    release_state};
+
+PyMODINIT_FUNC PyInit_hom_calls(void) { return PyModuleDef_Init(&module); }

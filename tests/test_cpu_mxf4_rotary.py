@@ -217,3 +217,31 @@ def test_a_failed_build_of_the_direct_calls_is_no_failed_build(tmp_path, monkeyp
     old.write_bytes(b"")
     build._build_calls(tmp_path, tmp_path / build.RUNNER_LIB.name, True, False)
     assert not old.exists() and "no such option" in capsys.readouterr().out
+
+
+def test_descriptors_of_a_derived_class_and_of_a_second_package(pkg, hom, nothing_launched):
+    """Both ways of calling take what is a MemRef by inheritance, and a package loaded a second time under another name
+    leaves the first one's calls as they were."""
+    import importlib.util
+    import sys
+    from pathlib import Path
+
+    class Named(pkg.MemRef):
+        pass
+
+    q, s = _coded(pkg, 5, 40)
+    x = Named(q.data_ptr, (5, 70))
+    path = Path(pkg.__file__)
+    spec = importlib.util.spec_from_file_location("hom_second", path, submodule_search_locations=[str(path.parent)])
+    second = importlib.util.module_from_spec(spec)
+    sys.modules["hom_second"] = second
+    try:
+        spec.loader.exec_module(second)
+        other = second.RunnerUtils()
+        assert second.MemRef is not pkg.MemRef
+        for h in (pkg.RunnerUtils(direct=False), hom):
+            _refused(pkg, 1, "need codes", h.homQuantizeMxF4F16, x, q, s)
+        with pytest.raises(second.HomError):
+            other.homQuantizeMxF4F16(second.MemRef(q.data_ptr, (5, 70)), *(second.MemRef(t.data_ptr, t.shape) for t in (q, s)))
+    finally:
+        del sys.modules["hom_second"]
