@@ -439,3 +439,51 @@ def test_quantize_transposed_with_a_long_k(hom, pkg, cuda, rows, dtype):
     rq, rs = ([v for v, _ in _buffers(pkg, cuda, rows, cols)])
     (hom.homQuantizeMxF4F16 if dtype == np.float16 else hom.homQuantizeMxF4F32)(to_dev(x.T, cuda), rq, rs)
     assert np.array_equal(rq.cpu().numpy(), q) and np.array_equal(rs.cpu().numpy(), s)
+
+
+@pytest.mark.parametrize("act,row", [(0, True), (1, False)])
+@pytest.mark.parametrize("m,n,k", [(1100, 2304, 768), (2500, 1024, 520), (3900, 2400, 300), (900, 1288, 2500), (9500, 264, 300),
+                                   (1001, 2001, 1060), (4001, 2390, 600), (300, 1000, 800), (2, 333, 5000)])
+def test_bias_without_gelu_and_residual_with_it(hom, cuda, m, n, k, act, row):
+    """An ordinary projection's row of C, and a matrix C under GELU, neither of them scaled."""
+    test_product_with_epilogue(hom, cuda, m, n, k, act, 1.0, 1.0, row)
+
+
+@pytest.mark.parametrize("declared", [False, True])
+@pytest.mark.parametrize("m,n,k", [(65536, 264, 1000), (65536, 263, 1000), (200000, 40, 1000), (66000, 600, 250),
+                                   (40000, 520, 1500), (70001, 258, 700)])
+def test_many_row_blocks_on_a_pair_are_exact(hom, cuda, m, n, k, declared):
+    """A pair that goes through three to eleven row blocks of A, kept in shared memory (K up to 1024) or not, and as many
+    turns of its accumulators and stages; the weight fetched early or not.  Sums as in the exact test above."""
+    import torch
+
+    rng = np.random.default_rng(m + n)
+    blocks = -(-k // 32)
+    coded, values = [], []
+    for rows in (m, n):
+        nibbles = rng.integers(0, 16, (rows, blocks * 32), dtype=np.uint8)
+        nibbles[:, k:] = 0
+        scales = np.zeros((-(-rows // 128), -(-blocks // 4), 512), np.uint8)
+        r, b = np.arange(rows)[:, None], np.arange(blocks)[None]
+        scales[r // 128, b // 4, r % 32 * 16 + r // 32 % 4 * 4 + b % 4] = 127
+        coded += [to_dev(nibbles[:, 0::2] | (nibbles[:, 1::2] << 4), cuda), to_dev(scales, cuda)]
+        table = np.concatenate([ref.VALUES, -ref.VALUES]).astype(np.float32)
+        values.append(table[nibbles])  # (sums of whole quarters below 2^24: exact in fp32 too)
+    want = values[0] @ values[1].T
+    assert np.abs(want).max() < 2 ** 16
+    row = rng.integers(-8, 9, (1, n)).astype(np.float16)
+    out, biased = (torch.full((m, n), 5.0, dtype=torch.float16, device=cuda) for _ in range(2))
+    torch.cuda.synchronize()
+    if declared:
+        for t in coded[2:]:
+            hom.declare_weights(t)
+    try:
+        hom.homGemmMxF4F16(*coded, None, out)
+        hom.homGemmMxF4F16(*coded, to_dev(row, cuda), biased, 0, 1.0, 1.0)
+        hom.synchronize()
+    finally:
+        if declared:
+            for t in coded[2:]:
+                hom.forget_weights(t)
+    assert np.array_equal(out.cpu().numpy(), want.astype(np.float16))
+    assert np.array_equal(biased.cpu().numpy(), (want + row.astype(np.float32)).astype(np.float16))

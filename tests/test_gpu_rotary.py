@@ -194,3 +194,30 @@ def test_rotary_on_another_stream_and_in_graphs(hom, cuda):
     finally:
         stream.synchronize()
         hom.use_torch_stream()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("bs,seq,heads,d,half", [(1, 1, 1, 4, 2), (2, 5, 3, 68, 34), (2, 3, 4, 50, 18), (1, 7, 5, 20, 2),
+                                                 (3, 11, 7, 100, 50), (1, 300, 12, 64, 10), (2, 2, 33, 36, 6)])
+def test_rotary_in_pieces_of_two_elements(hom, cuda, bs, seq, heads, d, half, interleaved, dtype):
+    test_rotary_layouts(hom, cuda, bs, seq, heads, d, half, interleaved, dtype)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("pitch,half", [(66, 32), (70, 16), (66, 24)])
+def test_rotary_heads_whose_pitch_allows_two_elements(hom, cuda, interleaved, dtype, pitch, half):
+    import torch
+
+    rng = np.random.default_rng(pitch + half)
+    store = torch.from_numpy(rng.standard_normal((3, 9, 5, pitch)).astype(dtype)).to(cuda)
+    view, before = store[..., :64], store.clone()
+    freq = _frequencies(half)
+    x = view.cpu().numpy()
+    out = torch.empty((3, 9, 5, 64), dtype=store.dtype, device=cuda)
+    call = _call(hom, store)
+    call(view, None, to_dev(freq, cuda), out, interleaved)
+    _check(out.cpu().numpy(), x, None, freq, interleaved, False, 1.0)
+    call(view, None, to_dev(freq, cuda), view, interleaved)  # in place: a lane keeps its turns where the pairs allow it
+    assert torch.equal(view, out) and torch.equal(store[..., 64:], before[..., 64:])
