@@ -302,20 +302,22 @@ void forget_constant_range(const void *ptr) {
   free_released_memory();
 }
 
-void withdraw_constant_ranges(const void *ptr, size_t bytes) {
-  const uintptr_t b = reinterpret_cast<uintptr_t>(ptr), e = b + bytes;
+void withdraw_constant_ranges(std::initializer_list<ByteRange> outputs) {
   bool any = false;
   {
     std::lock_guard<std::mutex> lock(g_const_mutex);
-    // from the last range that starts before the end, back to the first that ends before the start
-    while (!g_const_ranges.empty()) {
-      auto range = g_const_ranges.lower_bound(e);
-      if (range == g_const_ranges.begin()) break;
-      --range;
-      if (range->second <= b) break;
-      drop_derived(range->first, range->second);
-      g_const_ranges.erase(range);
-      any = true;
+    for (const ByteRange &output : outputs) {
+      const uintptr_t b = reinterpret_cast<uintptr_t>(output.ptr), e = b + output.bytes;
+      // from the last range that starts before the end, back to the first that ends before the start
+      while (!g_const_ranges.empty()) {
+        auto range = g_const_ranges.lower_bound(e);
+        if (range == g_const_ranges.begin()) break;
+        --range;
+        if (range->second <= b) break;
+        drop_derived(range->first, range->second);
+        g_const_ranges.erase(range);
+        any = true;
+      }
     }
   }
   if (any) free_released_memory();

@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <memory>
 
 #include <cuda_fp16.h>
@@ -81,9 +82,13 @@ cudaStream_t current_stream();
 // named through homDeclareWeights).
 void declare_constant_range(const void *ptr, size_t bytes);
 void forget_constant_range(const void *ptr);
-// For an entry point whose output may have been declared: what [ptr, ptr + bytes) touches is
-// constant no longer, from the coming launch on.
-void withdraw_constant_ranges(const void *ptr, size_t bytes);
+// For an entry point whose outputs may have been declared: what they touch is constant no longer,
+// from the coming launch on.
+struct ByteRange {
+  const void *ptr;
+  size_t bytes;
+};
+void withdraw_constant_ranges(std::initializer_list<ByteRange> outputs);
 bool is_constant_range(const void *ptr, size_t bytes);
 // For the lifetime of the object this thread may allocate, free and wait for a stream although some
 // other stream is being captured (the default capture mode refuses that, and breaks the capture, to

@@ -116,8 +116,7 @@ void quantize_entry(const char *name, int64_t rankX, void *dstX, bool transposed
     return;
   }
   // A product that requested these early would read them while they are written.
-  hom::withdraw_constant_ranges(Q.ptr, static_cast<size_t>(Q.numel()));
-  hom::withdraw_constant_ranges(S.ptr, static_cast<size_t>(S.numel()));
+  hom::withdraw_constant_ranges({{Q.ptr, static_cast<size_t>(Q.numel())}, {S.ptr, static_cast<size_t>(S.numel())}});
   mxf4::quantize(reinterpret_cast<const T *>(X.ptr), transposed, reinterpret_cast<uint8_t *>(Q.ptr),
                  reinterpret_cast<uint8_t *>(S.ptr), rows, cols, hom::current_stream());
 }

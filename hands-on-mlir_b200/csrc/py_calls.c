@@ -38,13 +38,15 @@ static int take(const State *state, Memrefs *m, PyObject *x) {
   m->descriptor[i] = NULL;
   m->made[i] = NULL;
   if (x == Py_None) return 1;
-  if (!state->memref_type) {
-    PyErr_SetString(PyExc_RuntimeError, "hom_calls: not bound");
-    return 0;
-  }
-  if (Py_TYPE(x) != state->memref_type && !PyType_IsSubtype(Py_TYPE(x), state->memref_type)) {
-    x = m->made[i] = PyObject_CallFunctionObjArgs(state->to_memref, x, NULL);
-    if (!x) return 0;
+  if (Py_TYPE(x) != state->memref_type) {
+    if (!state->memref_type) {
+      PyErr_SetString(PyExc_RuntimeError, "hom_calls: not bound");
+      return 0;
+    }
+    if (!PyType_IsSubtype(Py_TYPE(x), state->memref_type)) {
+      x = m->made[i] = PyObject_CallFunctionObjArgs(state->to_memref, x, NULL);
+      if (!x) return 0;
+    }
   }
   PyObject *rank = PyObject_GetAttr(x, state->s_rank);
   PyObject *address = rank ? PyObject_GetAttr(x, state->s_address) : NULL;
