@@ -5,6 +5,10 @@
 // 128 rows of B and the accumulator of its 128 output rows.  The grid is persistent.  A step is 256
 // values along K; its four 256 x 256 x 64 MMAs take 512 tensor-pipe cycles.
 //
+// The times in this file are those of a few calls in a burst.  In a loop that the power limit has
+// slowed down the long ones take more: 131072 x 4096 x 1024 with GELU 392 us instead of 324, 16384 x
+// 4096 x 4096 125 instead of 109, 131072 x 4096 x 256 with GELU 305 instead of 274.
+//
 // What bounds it: a step brings 35 KB to each SM, and with four stages in flight L2 delivers some
 // 16 TB/s.  Timed by leaving parts out, 16384 x 4096 x 4096 (107 us) takes 77 us with a quarter of
 // the MMAs and no stores, 74 with neither loads nor stores: the two overlap, but not wholly.  The
@@ -16,8 +20,9 @@
 // use, and their reads of the scales, are over.  Two whole accumulators do not fit beside 96 columns
 // of scales: the first lies in [0, 256), the second in [160, 416), and the warps that drain the 96
 // columns they share take them into registers at once, so that the next tile's MMAs can start while
-// the rest is drained beside them.  (192-column tiles need not share, but pull 13 % more through L2
-// for the same work: 16384 x 4096 x 4096 120 us instead of 107, 32768 x 4096 x 1024 73 instead of 69.)
+// the rest is drained beside them.  (192-column tiles need not share, but pull 1.18 times the bytes
+// through L2 for the same work, 31 KB a step instead of 35 for three quarters of the columns: 16384 x
+// 4096 x 4096 120 us instead of 107, 32768 x 4096 x 1024 73 instead of 69.)
 //
 // With GELU the epilogue's instructions are the bound where K is small: 131072 x 4096 x 256 takes
 // 277 us, 209 without GELU, the rate at which D can be written; 3400 of the 5300 cycles that a tile

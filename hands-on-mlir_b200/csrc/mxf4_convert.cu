@@ -201,9 +201,12 @@ struct ShiftedEight {
 // consecutive bytes of a scale tile.  A lane holds eight values, four lanes a block.  ALIGNED: rows
 // start on 16 bytes (cols % 8 == 0).  Otherwise, fp16: a lane reads the two 16-byte pieces that its
 // values lie in and moves them down, 20011 x 777 values 15.7 us, 37.9 element by element.  fp32: the
-// warp reads element by element, coalesced, and sorts the values through shared memory, 15.9 us; in
+// warp reads element by element, coalesced, and sorts the values through shared memory, 16.3 us; in
 // 16-byte pieces 24.5, and by 4-byte asynchronous copies 19.6.  (Slower too: a persistent form that
-// requests the next unit's values early, whose registers cost more loads in flight than it gains.)
+// requests the next unit's values early, whose registers cost more loads in flight than it gains; and
+// for fp16 one 16-byte piece a lane, the second by a shuffle from the neighbour, 21 to 28 us.)  The
+// memory would need 6.0 us for the fp16 values and 10.8 for the fp32 ones: a lane requests 32 bytes for
+// its 16, or single elements.
 //
 // What the rows kernel needs is many loads in flight, so its registers are held down: 65536 x 4096
 // fp16 values 119 us with room for five CTAs on an SM, 112 for eight (6.0 TB/s); 20011 x 776 fp32
@@ -304,8 +307,9 @@ quantize_rows_kernel(const Params p) {
 // x stored [cols, rows]: a thread owns one block of COLUMNS rows of the result, that is 32 values of
 // as many columns of x, all of them in flight; neighbouring threads read neighbouring elements.  A
 // CTA makes one scale tile, whose bytes it gathers in shared memory.  Two columns for fp16 (rows even,
-// x on 4 bytes): a [4096, 4096] weight takes 14.1 us (3.0 TB/s: pieces of 256 bytes out of rows of
-// 8 KB), with 2-byte loads 27.7.
+// x on 4 bytes): a [4096, 4096] weight takes 13.4 us (3.2 TB/s: pieces of 256 bytes out of rows of
+// 8 KB); with one column, 2-byte loads, 4097 rows of 4096 values 16.4.  fp32 [4096, 4096] 16.0 us, 4.7
+// TB/s (pieces of 512 bytes).
 //
 // The scale tiles along K are the grid's second dimension, which ends at 65535.  LONG: the third takes
 // what is beyond.  (An instantiation of its own: the loads are scheduled so finely that the additional
@@ -381,7 +385,9 @@ quantize_columns_kernel(const Params p) {
 
 // The way back, with the same division of work.  Where a lane's eight values are more than 16 bytes
 // (fp32), or rows start anywhere, they go through shared memory, so that a store of the warp covers
-// consecutive bytes (20011 x 776 fp32 values: two half-filled stores a lane 16.4 us).
+// consecutive bytes (20011 x 776 fp32 values 13.8 us, with two half-filled stores a lane 16.4).  fp16
+// 65536 x 4096 104.5 us, 6.5 TB/s, 4096 x 4096 8.5; rows that start anywhere are stored element by
+// element, 20011 x 777 fp16 values 13.9 us where the memory needs 6.0, fp32 ones 14.7 (10.8).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kWarps)
 dequantize_kernel(const Params p) {

@@ -81,10 +81,14 @@ __device__ __forceinline__ void apply_turns(Vec<T, VEC> &first, Vec<T, VEC> &sec
 // the same pairs of every head and keeps their sines and cosines in registers (64 x 512 tokens of 32
 // heads: 65 us without).
 //
-// Bound by memory where a token has many heads: each element is read and written once, 64 x 512 x 32
-// heads x 64 fp16 values in 41.1 us, 6.5 TB/s; otherwise by what a token costs (32 x 512 x 12 heads x
-// 128 32.5 us, 3.1 TB/s).  Four CTAs on an SM with two tasks a lane in flight; three CTAs with four took
-// 47 us, six with one 45.
+// Bound by memory where FIXED holds and the vectors have 16 bytes: each element is read and written
+// once, 64 x 512 tokens of 32 heads of 64 fp16 values in 41.1 us, 6.5 TB/s, 32 x 512 tokens of 24 heads
+// of 128 in 32.9, 6.1 TB/s.  Four CTAs on an SM with two tasks a lane in flight; three CTAs with four
+// took 47 us, six with one 45.  Otherwise by instructions, and by the few bytes that a lane has in
+// flight: every task finds its place and reads its sines from shared memory, for VEC pairs at a time.
+// 32 x 512 tokens of 24 fp16 heads, us, and the time that the memory needs: of 80 32.0 / 19.2, of 96
+// 36.6 / 23.1; by vectors of four elements of 72 36.5 / 17.3, of 88 43.2 / 21.2; of two of 68 52.7 /
+// 16.4, of 100 74 / 24; of one of 50 48.3 / 12.0.
 template <typename T, int VEC, bool INTERLEAVED, bool FIXED>
 __global__ void __launch_bounds__(32 * kWarps, 4) rotary_kernel(const Params p) {
   extern __shared__ float2 turns[];
