@@ -198,9 +198,8 @@ gemm_f16_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
       uint64_t da = da0, db = db0;
       uint32_t bar = full_bar(0), ph = 0;
       bool ok = true;
-      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       for (int i = 0; i < num_kb; ++i) {
-        ok = mbar_wait(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
+        ok = mbar_wait<true>(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
         if (!ok) break;
         tc_fence_after_sync();
         tc_mma_f16_ss(tmem_base, da, db, idesc, i != 0 ? 1u : 0u);

@@ -299,12 +299,12 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         else tma_load_3d_pair(dst + kCodeBytes, &tmSB, bar, 0, step * kStepTiles, n0 / kTileRows);
       };
       // The first round of stages is armed, and a declared B requested, before the previous kernel
-      // has finished; the ring's stages are free the first time round, so that no wait with a limit
-      // comes before the one for that kernel.
+      // has finished.  The stages are free the first time round: the producer of B waits for that
+      // kernel after it, before its first limited wait.
       int early = first < last ? min(kStages, p.steps) : 0, a_early = early;
       if (arms)
         for (int i = 0; i < early; ++i) mbar_arrive_expect_tx(armed_bar + 8 * i, armed_bytes);
-      bool waits = warp == 2 && p.b_early;  // still has the previous kernel to wait for
+      bool waits = warp == 2 && p.b_early;
       if (!waits) pdl_wait();
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
@@ -357,7 +357,6 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       uint32_t slot = 0, ph = 0, a_ph = 0;
       bool ok = true;
       int it = 0, n_block = first % p.n_blocks;  // (where A is resident)
-      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       for (int tile = first; tile < last && ok; tile += stride, ++it) {
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + (acc ? kSecondAcc : 0);
@@ -365,8 +364,8 @@ gemm_mxf4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (++n_block == p.n_blocks) n_block = 0;
         const bool ends_a = resident && (tile + 1 == last || n_block == 0);
         for (int i = 0; i < p.steps; ++i) {
-          ok = mbar_wait(full_bar(slot), ph, abort_flag, p.status, kDevWaitTimeoutMma);
-          if (ok && new_a) ok = mbar_wait(a_full_bar(i), a_ph, abort_flag, p.status, kDevWaitTimeoutMma);
+          ok = mbar_wait<true>(full_bar(slot), ph, abort_flag, p.status, kDevWaitTimeoutMma);
+          if (ok && new_a) ok = mbar_wait<true>(a_full_bar(i), a_ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (!ok) break;
           tc_fence_after_sync();
           const uint32_t src_a = smem_base + (resident ? i : slot) * kAStageBytes;

@@ -201,10 +201,9 @@ gemm_mxf4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       // the tile may start in the middle of a scale tile
       const uint32_t shift = n0 % kTileRows / 32;
       bool ok = true;
-      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        ok = mbar_wait(full_bar(s), (i / kStages) & 1, abort_flag, p.status, kDevWaitTimeoutMma);
+        ok = mbar_wait<true>(full_bar(s), (i / kStages) & 1, abort_flag, p.status, kDevWaitTimeoutMma);
         if (!ok) break;
         tc_fence_after_sync();
         const uint32_t src = smem_base + s * kStageBytes;

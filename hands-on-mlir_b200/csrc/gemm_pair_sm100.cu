@@ -249,7 +249,6 @@ gemm_f16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       uint32_t bar = full_bar(0), ph = 0;
       bool ok = true;
       int it = 0;
-      pdl_wait();  // no limit runs while the previous kernel does (gemm_sm100.cu)
       HOM_DIAG(long long t_full = 0, t_acc = 0; const long long t_begin = clock64();)
       for (int unit = pair; unit < p.num_units && ok; unit += num_pairs, ++it) {
         const int part = unit % p.split_k;
@@ -264,7 +263,7 @@ gemm_f16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const uint32_t d_tmem = tmem_base + acc * BN2;
         for (int kb = 0; kb < num_kb; ++kb) {
           HOM_DIAG(const long long tw = p.prof ? clock64() : 0;)
-          ok = mbar_wait(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
+          ok = mbar_wait<true>(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (!ok) break;
           HOM_DIAG(if (p.prof) t_full += clock64() - tw;)
           tc_fence_after_sync();

@@ -212,7 +212,7 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       // waiting for the previous kernel: the first ring of B tiles then arrives while that one
       // finishes.  A B of unknown origin only after.  (Its bytes may land before the A warp has
       // armed the barrier: the phase cannot complete without that arrival.)  The ring's stages are
-      // free the first time round, so no wait with a limit comes before the one for that kernel.
+      // free the first time round, so that no limited wait comes before the one for that kernel.
       bool early = p.b_early != 0;
       if (!early) pdl_wait();
       for (int unit = blockIdx.x; unit < p.num_units && ok; unit += gridDim.x) {
@@ -265,7 +265,6 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       uint32_t bar = full_bar(0), ph = 0;
       bool ok = true;
       int it = 0;
-      pdl_wait();  // the limits of the waits below are for this kernel's work, not for the previous one's
       HOM_DIAG(long long t_full = 0, t_acc = 0; const long long t_begin = clock64();)
       for (int unit = blockIdx.x; unit < p.num_units && ok; unit += gridDim.x, ++it) {
         const int part = unit % p.split_k;
@@ -280,7 +279,7 @@ gemm_f16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const uint32_t d_tmem = tmem_base + acc * BN;
         for (int kb = 0; kb < num_kb; ++kb) {
           HOM_DIAG(const long long tw = p.prof ? clock64() : 0;)
-          ok = mbar_wait(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
+          ok = mbar_wait<true>(bar, ph, abort_flag, p.status, kDevWaitTimeoutMma);
           if (!ok) break;
           HOM_DIAG(if (p.prof) t_full += clock64() - tw;)
           tc_fence_after_sync();
